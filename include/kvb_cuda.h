@@ -322,6 +322,144 @@ typedef struct kvb_peer_barrier_args {
 } kvb_peer_barrier_args;
 int kvb_peer_barrier_async(const kvb_peer_barrier_args* args, void* workspace, void* stream);
 
+/* ---- serving steps of several new tokens per sequence -------------------------------------- */
+/* No counterpart in the reference, which decodes one token per sequence from caches written before
+ * the run. A serving step that prefills prompts (whole, or in chunks) or verifies drafted tokens is
+ *   kvb_step_plan      pages and slots of the new tokens, from the requests' lengths,
+ *   kvb_paged_append   their keys and values into those pages,
+ *   kvb_paged_chunk_async   attention of the new tokens over the pages (after the append), or
+ *   kvb_prompt_async   attention over whole prompts straight from the projections' output.
+ * All are stream-ordered on the current device, read nothing on the host, allocate nothing and can
+ * be captured in a CUDA graph. The step's tokens are packed: sequence b owns rows
+ * cu_new[b] .. cu_new[b + 1) (cu_new[0] = 0). Rows behind cu_new[batch] are not written. */
+
+/* The step plan. Sequence b has seq_lens[b] tokens cached and adds new_lens[b]; its pages so far are in
+ * the block table. Free block ids are ring[head % ring_size], ring[(head + 1) % ring_size], ... up to
+ * tail (ring_pos = {head, tail}, 0 <= tail - head <= ring_size); a finished request's ids are put back
+ * by writing them at tail and raising it. The plan takes the pages that the new tokens open, in
+ * sequence order, and writes:
+ *   block_table   the ids of the new pages (other entries are left as they were);
+ *   total_lens    seq_lens + new_lens, or -1 for a sequence that was refused;
+ *   cu_new        the packed starts, new_lens summed (never above num_tokens);
+ *   slot_map      per token id * page_size + place in the page; -1 for tokens of a refused sequence and
+ *                 behind the last token;
+ *   positions     per token its position in its sequence, 0 behind the last token (may be NULL);
+ *   ring_out      {head after the step, tail}.
+ * Refused are: a negative length, a total above max_blocks * page_size, tokens beyond num_tokens (bit 1
+ * of error_word), and, in order, the sequences whose pages the ring cannot give any more (bit 2; a
+ * sequence that opens no page is still served). A ring or table id outside [0, num_blocks) gives its
+ * tokens slot -1 and bit 2; a ring_pos outside its bounds counts as an empty ring (bit 8). Outputs must
+ * not overlap inputs (block_table, which is both, apart). */
+typedef struct kvb_step_plan_args {
+    int batch, page_size, max_blocks;
+    int num_tokens;           /* entries of slot_map and positions */
+    const int32_t* seq_lens;  /* [batch] */
+    const int32_t* new_lens;  /* [batch] */
+    int32_t* block_table;     /* [batch][max_blocks] */
+    const int32_t* ring;      /* [ring_size] */
+    const int64_t* ring_pos;  /* [2] */
+    int64_t* ring_out;        /* [2] */
+    int32_t* total_lens;      /* [batch] */
+    int32_t* cu_new;          /* [batch + 1] */
+    int64_t* slot_map;        /* [num_tokens] */
+    int32_t* positions;       /* [num_tokens] or NULL */
+    int64_t ring_size, num_blocks;
+    unsigned int* error_word; /* optional device word, bits are OR-ed in */
+} kvb_step_plan_args;
+int kvb_step_plan(const kvb_step_plan_args* args, void* stream);
+
+/* The append: token t's K and V rows (k + t * k_stride, num_kv_heads x head_dim elements, fp32 or fp16)
+ * into the pages.
+ * fp32 and fp16 pools: to slot slot_map[t], rounded to nearest where the pool is fp16 and the rows are
+ *   fp32 (fp16 rows into an fp32 pool are refused). Slot -1 skips the token; any other slot outside
+ *   the pool skips it and sets bit 2. No slot may be given twice.
+ * int8 pools: through the block table, since a page's scale depends on all its rows. Per (page touched,
+ *   KV head), with amax the largest |x| of the new rows in it, s = amax / 127 (fp32), or the page's
+ *   scale so far where that is larger and the page held rows before; those rows are rounded again,
+ *   rint(q * (s_old / s)), when the scale grew; new rows are clamp(rint(x / s), -127, 127), 0 for s = 0.
+ *   Rows of a page from its first slot on in one append give what kvb_quantize_paged_i8 gives. A
+ *   sequence with total_lens -1 is skipped; one whose total is below its new tokens or above
+ *   max_blocks * page_size is skipped with bit 1; a block id outside the pool skips its page with bit
+ *   2. A page may belong to one appending sequence only.
+ * k, v and the pools 16-byte aligned, strides whole multiples of 16 bytes, head_dim a multiple of 8. */
+typedef struct kvb_append_args {
+    kvb_shape shape;          /* batch (int8), num_kv_heads, head_dim; num_heads unused */
+    int src_type;             /* KVB_F32 or KVB_F16 */
+    int kv_type;              /* pool type */
+    int page_size, max_blocks;
+    int num_tokens;
+    const void* k;
+    const void* v;
+    int64_t k_stride, v_stride;   /* elements between tokens */
+    void* k_pool;             /* [num_blocks][num_kv_heads][page_size][head_dim] */
+    void* v_pool;
+    float* k_scale;           /* int8: [num_blocks][num_kv_heads] */
+    float* v_scale;
+    int64_t num_blocks;
+    const int64_t* slot_map;  /* fp32, fp16 pools: [num_tokens] */
+    const int32_t* block_table;   /* int8: [batch][max_blocks] */
+    const int32_t* total_lens;    /* int8: [batch], the new tokens included */
+    const int32_t* cu_new;        /* int8: [batch + 1] */
+    unsigned int* error_word; /* optional */
+} kvb_append_args;
+int kvb_paged_append(const kvb_append_args* args, void* stream);
+
+/* Attention of the step's new tokens over the paged cache, which holds them already: sequence b's new
+ * token i, at position total_lens[b] - n_b + i, sees the tokens at positions up to its own. Head
+ * layouts, pools, scales and the softmax scale are those of kvb_paged_decode_async; one new token per
+ * sequence is its decode step. q and out are both fp32 (fp32-level results) or both fp16 (the
+ * probabilities are rounded to fp16 for the value product; sums and maxima are fp32).
+ * Values behind a sequence's last token are never used, whatever bits they hold; a non-finite key or
+ * value reaches the tokens that see it and no other.
+ * max_new and max_len bound the new tokens and the total of any sequence (they size the grid). A
+ * sequence that exceeds them, whose total is below its new tokens or above max_blocks * page_size (a
+ * total of -1 from the plan, too), or that has rows outside [0, num_tokens), gets NaN rows and sets bit
+ * 1; a live block id outside the pool NaN rows and bit 2. error_word is required: zero it once, read
+ * it when convenient. The workspace needs no preparation and holds nothing between calls. At most 64
+ * query heads per KV head. q 16-byte aligned with a stride of whole 16 bytes, out 16-byte aligned. */
+typedef struct kvb_chunk_args {
+    kvb_shape shape;
+    int q_type;               /* KVB_F32 or KVB_F16: q and out */
+    int kv_type;
+    int page_size, max_blocks;
+    int num_tokens, max_new, max_len;
+    const void* q;            /* [num_tokens][num_heads][head_dim], q_stride elements between tokens */
+    int64_t q_stride;
+    const void* k;            /* pools */
+    const void* v;
+    const float* k_scale;
+    const float* v_scale;
+    int64_t num_blocks;
+    const int32_t* block_table;
+    const int32_t* total_lens;    /* [batch], the new tokens included */
+    const int32_t* cu_new;        /* [batch + 1] */
+    void* out;                /* [num_tokens][num_heads][head_dim] */
+    unsigned int* error_word;
+    int kernel;               /* KVB_KERNEL_AUTO, _SIMT or _UMMA */
+} kvb_chunk_args;
+int kvb_paged_chunk_workspace_bytes(const kvb_chunk_args* args, size_t* bytes);
+int kvb_paged_chunk_async(const kvb_chunk_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Causal attention over whole packed prompts, q, k, v and out all fp32 or all fp16: token i of a prompt
+ * sees its tokens 0 .. i. k and v need not be in pages: they are rows of the projections' output
+ * (num_kv_heads x head_dim elements per token, strides in elements, whole multiples of 16 bytes). Bounds, refusals,
+ * alignment and the workspace as in kvb_paged_chunk_async, max_len bounding a prompt's tokens. */
+typedef struct kvb_prompt_args {
+    kvb_shape shape;
+    int type;                 /* KVB_F32 or KVB_F16 */
+    int num_tokens, max_len;
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t q_stride, k_stride, v_stride;
+    const int32_t* cu_lens;   /* [batch + 1] */
+    void* out;
+    unsigned int* error_word;
+    int kernel;
+} kvb_prompt_args;
+int kvb_prompt_workspace_bytes(const kvb_prompt_args* args, size_t* bytes);
+int kvb_prompt_async(const kvb_prompt_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -34,6 +34,8 @@ __all__ = [
     "paged_workspace_bytes", "paged_part_tokens", "paged_part_tokens_for", "paged_decode_async", "paged_error_flag",
     "paged_decode_static", "paged_static_error_flag", "library_path", "lib", "MAX_PEERS", "ipc_alloc", "ipc_free",
     "ipc_open", "ipc_close", "peer_out", "paged_decode_gather_async", "peer_barrier_args", "peer_barrier_async",
+    "step_plan_args", "step_plan", "append_args", "paged_append", "chunk_args", "paged_chunk_workspace_bytes",
+    "paged_chunk_async", "prompt_args", "prompt_workspace_bytes", "prompt_async",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -520,3 +522,120 @@ def peer_barrier_async(b: _CPeerBarrierArgs, workspace: int, stream: int = 0) ->
     """kvb_peer_barrier_async: the step barrier after paged_decode_gather_async on every rank; a wait
     that runs out sets bit 4 of the workspace's error word."""
     _check(_c_peer_barrier(ctypes.byref(b), workspace or None, stream or None), "peer_barrier_async")
+
+
+# ---- serving steps of several new tokens per sequence (include/kvb_cuda.h) --------------------------
+
+_P = ctypes.c_void_p
+
+
+class _CStepPlanArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int), ("page_size", ctypes.c_int), ("max_blocks", ctypes.c_int),
+                ("num_tokens", ctypes.c_int), ("seq_lens", _P), ("new_lens", _P), ("block_table", _P), ("ring", _P),
+                ("ring_pos", _P), ("ring_out", _P), ("total_lens", _P), ("cu_new", _P), ("slot_map", _P),
+                ("positions", _P), ("ring_size", ctypes.c_int64), ("num_blocks", ctypes.c_int64), ("error_word", _P)]
+
+
+class _CAppendArgs(ctypes.Structure):
+    _fields_ = [("shape", _CShape), ("src_type", ctypes.c_int), ("kv_type", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("max_blocks", ctypes.c_int), ("num_tokens", ctypes.c_int), ("k", _P),
+                ("v", _P), ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64), ("k_pool", _P),
+                ("v_pool", _P), ("k_scale", _P), ("v_scale", _P), ("num_blocks", ctypes.c_int64), ("slot_map", _P),
+                ("block_table", _P), ("total_lens", _P), ("cu_new", _P), ("error_word", _P)]
+
+
+class _CChunkArgs(ctypes.Structure):
+    _fields_ = [("shape", _CShape), ("q_type", ctypes.c_int), ("kv_type", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("max_blocks", ctypes.c_int), ("num_tokens", ctypes.c_int), ("max_new", ctypes.c_int),
+                ("max_len", ctypes.c_int), ("q", _P), ("q_stride", ctypes.c_int64), ("k", _P), ("v", _P),
+                ("k_scale", _P), ("v_scale", _P), ("num_blocks", ctypes.c_int64), ("block_table", _P),
+                ("total_lens", _P), ("cu_new", _P), ("out", _P), ("error_word", _P), ("kernel", ctypes.c_int)]
+
+
+class _CPromptArgs(ctypes.Structure):
+    _fields_ = [("shape", _CShape), ("type", ctypes.c_int), ("num_tokens", ctypes.c_int), ("max_len", ctypes.c_int),
+                ("q", _P), ("k", _P), ("v", _P), ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64),
+                ("v_stride", ctypes.c_int64), ("cu_lens", _P), ("out", _P), ("error_word", _P),
+                ("kernel", ctypes.c_int)]
+
+
+_c_step_plan = _sig("kvb_step_plan", ctypes.c_int, ctypes.POINTER(_CStepPlanArgs), _P)
+_c_append = _sig("kvb_paged_append", ctypes.c_int, ctypes.POINTER(_CAppendArgs), _P)
+_c_chunk_ws = _sig("kvb_paged_chunk_workspace_bytes", ctypes.c_int, ctypes.POINTER(_CChunkArgs),
+                   ctypes.POINTER(ctypes.c_size_t))
+_c_chunk = _sig("kvb_paged_chunk_async", ctypes.c_int, ctypes.POINTER(_CChunkArgs), _P, ctypes.c_size_t, _P)
+_c_prompt_ws = _sig("kvb_prompt_workspace_bytes", ctypes.c_int, ctypes.POINTER(_CPromptArgs),
+                    ctypes.POINTER(ctypes.c_size_t))
+_c_prompt = _sig("kvb_prompt_async", ctypes.c_int, ctypes.POINTER(_CPromptArgs), _P, ctypes.c_size_t, _P)
+
+
+def step_plan_args(batch: int, page_size: int, max_blocks: int, num_tokens: int, *, seq_lens: int, new_lens: int,
+                   block_table: int, ring: int, ring_pos: int, ring_out: int, total_lens: int, cu_new: int,
+                   slot_map: int, ring_size: int, num_blocks: int, positions: int = 0,
+                   error_word: int = 0) -> _CStepPlanArgs:
+    """kvb_step_plan_args over raw device pointers (ints)."""
+    return _CStepPlanArgs(batch, page_size, max_blocks, num_tokens, seq_lens, new_lens, block_table, ring, ring_pos,
+                          ring_out, total_lens, cu_new, slot_map, positions or None, ring_size, num_blocks,
+                          error_word or None)
+
+
+def step_plan(a: _CStepPlanArgs, stream: int = 0) -> None:
+    """kvb_step_plan: pages, slots, positions and packed starts of a step's new tokens."""
+    _check(_c_step_plan(ctypes.byref(a), stream or None), "step_plan")
+
+
+def append_args(batch: int, num_kv_heads: int, head_dim: int, src_type: KvType, kv_type: KvType, page_size: int,
+                num_tokens: int, *, k: int, v: int, k_stride: int, v_stride: int, k_pool: int, v_pool: int,
+                num_blocks: int, slot_map: int = 0, k_scale: int = 0, v_scale: int = 0, max_blocks: int = 0,
+                block_table: int = 0, total_lens: int = 0, cu_new: int = 0, error_word: int = 0) -> _CAppendArgs:
+    """kvb_append_args over raw device pointers (ints); strides in elements."""
+    return _CAppendArgs(_CShape(batch, num_kv_heads, num_kv_heads, head_dim), int(src_type), int(kv_type), page_size,
+                        max_blocks, num_tokens, k or None, v or None, k_stride, v_stride, k_pool or None,
+                        v_pool or None, k_scale or None, v_scale or None, num_blocks, slot_map or None,
+                        block_table or None, total_lens or None, cu_new or None, error_word or None)
+
+
+def paged_append(a: _CAppendArgs, stream: int = 0) -> None:
+    """kvb_paged_append: the new tokens' keys and values into their pages."""
+    _check(_c_append(ctypes.byref(a), stream or None), "paged_append")
+
+
+def chunk_args(shape: Shape, q_type: KvType, kv_type: KvType, page_size: int, max_blocks: int, num_tokens: int,
+               max_new: int, max_len: int, *, q: int, q_stride: int, k: int, v: int, num_blocks: int,
+               block_table: int, total_lens: int, cu_new: int, out: int, error_word: int, k_scale: int = 0,
+               v_scale: int = 0, kernel: Kernel = Kernel.auto) -> _CChunkArgs:
+    """kvb_chunk_args over raw device pointers (ints); q_stride in elements."""
+    return _CChunkArgs(shape._c(), int(q_type), int(kv_type), page_size, max_blocks, num_tokens, max_new, max_len,
+                       q or None, q_stride, k or None, v or None, k_scale or None, v_scale or None, num_blocks,
+                       block_table or None, total_lens or None, cu_new or None, out or None, error_word or None,
+                       int(kernel))
+
+
+def paged_chunk_workspace_bytes(a: _CChunkArgs) -> int:
+    n = ctypes.c_size_t()
+    _check(_c_chunk_ws(ctypes.byref(a), ctypes.byref(n)), "paged_chunk_workspace_bytes")
+    return n.value
+
+
+def paged_chunk_async(a: _CChunkArgs, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+    """kvb_paged_chunk_async: attention of a step's new tokens over the paged cache."""
+    _check(_c_chunk(ctypes.byref(a), workspace or None, int(workspace_bytes), stream or None), "paged_chunk_async")
+
+
+def prompt_args(shape: Shape, type: KvType, num_tokens: int, max_len: int, *, q: int, k: int, v: int, q_stride: int,
+                k_stride: int, v_stride: int, cu_lens: int, out: int, error_word: int,
+                kernel: Kernel = Kernel.auto) -> _CPromptArgs:
+    """kvb_prompt_args over raw device pointers (ints); strides in elements."""
+    return _CPromptArgs(shape._c(), int(type), num_tokens, max_len, q or None, k or None, v or None, q_stride,
+                        k_stride, v_stride, cu_lens or None, out or None, error_word or None, int(kernel))
+
+
+def prompt_workspace_bytes(a: _CPromptArgs) -> int:
+    n = ctypes.c_size_t()
+    _check(_c_prompt_ws(ctypes.byref(a), ctypes.byref(n)), "prompt_workspace_bytes")
+    return n.value
+
+
+def prompt_async(a: _CPromptArgs, workspace: int, workspace_bytes: int, stream: int = 0) -> None:
+    """kvb_prompt_async: causal attention over whole packed prompts."""
+    _check(_c_prompt(ctypes.byref(a), workspace or None, int(workspace_bytes), stream or None), "prompt_async")

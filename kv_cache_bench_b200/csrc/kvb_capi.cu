@@ -20,6 +20,7 @@
 
 #include "../../include/kvb_cuda.h"
 #include "kvb_internal.h"
+#include "kvb_step.h"
 
 namespace {
 
@@ -443,6 +444,45 @@ int end_timed(State& S, cudaEvent_t e0, cudaEvent_t e1, double* ms, bool check) 
 }
 
 }  // namespace
+
+// ---- shared with kvb_step_capi.cu ------------------------------------------------------------------
+
+int kvb_fail(int code, const char* msg) {
+    try {
+        return fail(code, msg);
+    } catch (...) {  // no memory for the text: the code still tells
+        return code;
+    }
+}
+
+int kvb_device_sms(int* num_sms) {
+    DeviceFacts f;
+    try {
+        if (int rc = device_facts(&f)) return rc;
+    } catch (...) {
+        return KVB_ERR_DEVICE;
+    }
+    *num_sms = f.num_sms;
+    return KVB_OK;
+}
+
+bool kvb_encode_tile_map(void* map, const void* base, int elem_size, int rank, const unsigned long long* dims,
+                         const unsigned long long* strides, const unsigned* box) {
+    PFN_cuTensorMapEncodeTiled_v12000 enc = encode_fn();
+    if (!enc) return false;
+    cuuint64_t d[3] = {1, 1, 1}, s[2] = {0, 0};
+    cuuint32_t b[3] = {1, 1, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    for (int i = 0; i < rank; ++i) {
+        d[i] = dims[i];
+        b[i] = box[i];
+        if (i) s[i - 1] = strides[i - 1];
+    }
+    return enc(static_cast<CUtensorMap*>(map),
+               elem_size == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t)rank,
+               const_cast<void*>(base), d, s, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 // ==================================================================================================
 extern "C" {

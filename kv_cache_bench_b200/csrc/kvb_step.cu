@@ -1,0 +1,422 @@
+// The two steps in front of attention when a serving step adds several tokens per sequence:
+//
+//   plan    which physical page and slot every new token of the step gets. With len_b tokens cached
+//           and n_b new ones, pages of P tokens:
+//             cu_b   = n_0 + ... + n_(b-1)                    (where b's tokens start in the packed step)
+//             have_b = ceil(len_b / P), need_b = ceil((len_b + n_b) / P) - have_b
+//             E_b    = need_0 + ... + need_b
+//           Sequence b's i-th new page is free id ring[(head + E_b - need_b + i) mod ring_size]; a
+//           sequence is served when its pages fit (need_b = 0 or E_b <= tail - head), so the served
+//           sequences that need pages are the first ones, and the result does not depend on timing.
+//   append  the new tokens' K and V rows written into those pages (fp32, fp16), or quantized into
+//           int8 pages with one scale per (page, KV head).
+//
+// No counterpart in the reference, whose block tables are built on the host before the run
+// (src/reference.cpp:11-30) and whose caches are written whole (src/reference.hpp:60-68,
+// src/reference.cpp:32-51).
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "kvb_device.cuh"
+#include "kvb_step.h"
+
+namespace {
+
+using namespace kvb_dev;
+
+// ---- plan ---------------------------------------------------------------------------------------
+
+constexpr int PL_THREADS = 512;
+constexpr int PL_WARPS = PL_THREADS / 32;
+
+struct Pair {
+    long long tok, blk;
+};
+
+// Every CTA scans the lengths (one sequence per thread and round) and then writes the slots of its own
+// range of tokens; CTA 0 also writes what belongs to the sequences. Nothing passes between CTAs, so
+// one launch does it all and B lengths are read once per CTA from L2. Bound by latency: two dependent
+// loads, a block scan and a store.
+__global__ void __launch_bounds__(PL_THREADS) step_plan_kernel(const PlanParams p) {
+    __shared__ int s_cu[PL_THREADS + 1];        // first token of a sequence of this round
+    __shared__ int s_len[PL_THREADS], s_have[PL_THREADS];
+    __shared__ long long s_first[PL_THREADS];   // ring position of its first new page; -1: not served
+    __shared__ Pair s_warp[PL_WARPS];
+    __shared__ unsigned long long s_head;
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    pdl_wait();
+    pdl_trigger();
+    long long head = __ldg(p.ring_pos), avail = __ldg(p.ring_pos + 1) - head;
+    if (head < 0 || avail < 0 || avail > p.ring_size) {
+        if (blockIdx.x == 0 && tid == 0 && p.error_flag) raise_error(p.error_flag, KVB_DEVERR_STATE);
+        head = max(head, 0ll);
+        avail = 0;
+    }
+    const long long head0 = p.ring_size > 0 ? head % p.ring_size : 0;
+    const long long capacity = min((long long)p.max_blocks * p.page, 0x7fffffffll);
+    const int per = int(((long long)p.num_tokens + gridDim.x - 1) / gridDim.x);
+    const int t0 = int(min((long long)p.num_tokens, (long long)blockIdx.x * per));
+    const int t1 = int(min((long long)p.num_tokens, (long long)t0 + per));
+    if (tid == 0) s_head = 0;
+    long long tok = 0, blk = 0;  // totals of the rounds before
+    unsigned bad = 0;
+    for (int b0 = 0; b0 < p.B; b0 += PL_THREADS) {
+        if (blockIdx.x != 0 && tok >= t1) break;
+        const int b = b0 + tid;
+        int len = 0, n = 0, have = 0, need = 0;
+        bool valid = false;
+        if (b < p.B) {
+            len = __ldg(p.seq_lens + b);
+            n = __ldg(p.new_lens + b);
+            valid = len >= 0 && n >= 0 && (long long)len + n <= capacity;
+            n = max(n, 0);
+            if (valid) {
+                have = len == 0 ? 0 : kvb_div(len - 1, p.div_page) + 1;
+                need = (len + n == 0 ? 0 : kvb_div(len + n - 1, p.div_page) + 1) - have;
+            }
+        }
+        Pair v{n, need};
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long a = __shfl_up_sync(0xffffffffu, v.tok, o), c = __shfl_up_sync(0xffffffffu, v.blk, o);
+            if (lane >= o) v.tok += a, v.blk += c;
+        }
+        __syncthreads();  // the round before is done with the shared arrays
+        if (lane == 31) s_warp[w] = v;
+        __syncthreads();
+        long long all_tok = 0, all_blk = 0;
+#pragma unroll
+        for (int i = 0; i < PL_WARPS; ++i) {
+            const Pair x = s_warp[i];
+            if (i < w) v.tok += x.tok, v.blk += x.blk;
+            all_tok += x.tok, all_blk += x.blk;
+        }
+        const long long end = tok + v.tok, start = end - n;  // exclusive and inclusive token sums
+        const long long E = blk + v.blk;
+        const bool served = valid && end <= p.num_tokens && (need == 0 || E <= avail);
+        const int cut = int(min(start, (long long)p.num_tokens));
+        s_cu[tid] = cut;
+        s_len[tid] = valid ? len : 0;
+        s_have[tid] = have;
+        s_first[tid] = served ? E - need : -1;
+        if (tid == PL_THREADS - 1) s_cu[PL_THREADS] = int(min(end, (long long)p.num_tokens));
+        if (blockIdx.x == 0 && b < p.B) {
+            p.total_lens[b] = served ? len + n : -1;
+            p.cu_new[b] = cut;
+            if (b == p.B - 1) p.cu_new[p.B] = int(min(end, (long long)p.num_tokens));
+            if (!valid || end > p.num_tokens) bad |= KVB_DEVERR_LENGTH;
+            else if (!served) bad |= KVB_DEVERR_BLOCK;
+            if (served && need > 0) atomicMax(&s_head, (unsigned long long)E);
+        }
+        __syncthreads();
+        // this round's tokens in the CTA's range
+        const int a = max(t0, int(min(tok, (long long)p.num_tokens)));
+        const int z = min(t1, int(min(tok + all_tok, (long long)p.num_tokens)));
+        for (int t = a + tid; t < z; t += PL_THREADS) {
+            int lo = 0, hi = PL_THREADS - 1;  // the last sequence that starts at or before t
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (s_cu[mid] <= t) lo = mid;
+                else hi = mid - 1;
+            }
+            const int pos = s_len[lo] + (t - s_cu[lo]);
+            const long long first = s_first[lo];
+            long long slot = -1;
+            if (first >= 0) {
+                const int pg = kvb_div(pos, p.div_page), at = pos - pg * p.page, fresh = pg - s_have[lo];
+                int* entry = p.block_table + (size_t)(b0 + lo) * p.max_blocks + pg;
+                int id;
+                if (fresh >= 0) {
+                    long long r = head0 + first + fresh;  // below twice the ring's size
+                    if (r >= p.ring_size) r -= p.ring_size;
+                    id = __ldg(p.ring + r);
+                    if (at == 0) *entry = id;
+                } else {
+                    id = *entry;
+                }
+                if (id >= 0 && id < p.num_blocks) slot = (long long)id * p.page + at;
+                else bad |= KVB_DEVERR_BLOCK;
+            }
+            p.slot_map[t] = slot;
+            if (p.positions) p.positions[t] = pos;
+        }
+        tok += all_tok;
+        blk += all_blk;
+    }
+    // entries behind the last token
+    for (long long t = max((long long)t0, tok) + tid; t < t1; t += PL_THREADS) {
+        p.slot_map[t] = -1;
+        if (p.positions) p.positions[t] = 0;
+    }
+    if (blockIdx.x == 0) {
+        __syncthreads();
+        if (tid == 0) {
+            p.ring_out[0] = __ldg(p.ring_pos) + (long long)s_head;
+            p.ring_out[1] = __ldg(p.ring_pos + 1);
+            if (p.B == 0) p.cu_new[0] = 0;
+        }
+    }
+    if (bad && p.error_flag) raise_error(p.error_flag, bad);
+}
+
+// ---- append -------------------------------------------------------------------------------------
+
+constexpr int AP_THREADS = 256;
+constexpr int AP_UNROLL = 4;  // pieces in flight per thread
+
+// fp32 and fp16 pools: a row of D values is DW = D * sizeof(DST) / 16 pieces of 16 destination bytes.
+// One thread moves one piece (several per loop round, so that their loads overlap); consecutive threads
+// take consecutive pieces, so both sides are read and written in whole lines. Bound by memory.
+template <typename SRC, typename DST>
+__global__ void __launch_bounds__(AP_THREADS) append_rows_kernel(const AppendParams p) {
+    constexpr int PER = 16 / sizeof(DST);  // values per piece
+    const int which = blockIdx.y;
+    const SRC* src = static_cast<const SRC*>(p.src[which]);
+    DST* pool = static_cast<DST*>(p.pool[which]);
+    const long long per_token = (long long)p.Hkv * p.div_row.d;
+    const long long total = per_token * p.num_tokens, limit = p.num_blocks * p.page;
+    const long long step = (long long)gridDim.x * AP_THREADS;
+    pdl_wait();
+    pdl_trigger();
+    for (long long i0 = (long long)blockIdx.x * AP_THREADS + threadIdx.x; i0 < total; i0 += AP_UNROLL * step) {
+        long long dst[AP_UNROLL];
+        uint4 raw[AP_UNROLL][sizeof(SRC) / sizeof(DST) > 1 ? 2 : 1];
+#pragma unroll
+        for (int u = 0; u < AP_UNROLL; ++u) {
+            const long long i = i0 + u * step;
+            dst[u] = -1;
+            if (i >= total) continue;
+            // a token's pieces are below 2^31 (checked by the host)
+            const long long t = i / per_token;
+            const int in = int(i - t * per_token), h = kvb_div(in, p.div_row), c = in - h * int(p.div_row.d);
+            const long long slot = __ldg(p.slot_map + t);
+            if (slot < 0 || slot >= limit) {
+                if (slot != -1 && p.error_flag) raise_error(p.error_flag, KVB_DEVERR_BLOCK);
+                continue;
+            }
+            long long block, at;
+            if (slot < (1ll << 31)) {
+                block = kvb_div(int(slot), p.div_page);
+                at = slot - block * p.page;
+            } else {
+                block = slot / p.page;
+                at = slot - block * p.page;
+            }
+            dst[u] = ((block * p.Hkv + h) * p.page + at) * p.D + c * PER;
+            const uint4* s = reinterpret_cast<const uint4*>(src + t * p.stride[which] + (long long)h * p.D + c * PER);
+            raw[u][0] = __ldcs(s);
+            if constexpr (sizeof(SRC) > sizeof(DST)) raw[u][1] = __ldcs(s + 1);
+        }
+#pragma unroll
+        for (int u = 0; u < AP_UNROLL; ++u) {
+            if (dst[u] < 0) continue;
+            uint4 out = raw[u][0];
+            if constexpr (sizeof(SRC) > sizeof(DST)) {  // fp32 rows into fp16 pages: one rounding to nearest
+                const float* f = reinterpret_cast<const float*>(&raw[u][0]);
+                const float* g = reinterpret_cast<const float*>(&raw[u][1]);
+                out.x = h2_as_u32(__floats2half2_rn(f[0], f[1]));
+                out.y = h2_as_u32(__floats2half2_rn(f[2], f[3]));
+                out.z = h2_as_u32(__floats2half2_rn(g[0], g[1]));
+                out.w = h2_as_u32(__floats2half2_rn(g[2], g[3]));
+            }
+            *reinterpret_cast<uint4*>(pool + dst[u]) = out;
+        }
+    }
+}
+
+template <typename SRC>
+__device__ __forceinline__ float4 load4(const SRC* s) {
+    if constexpr (sizeof(SRC) == 4) {
+        return __ldg(reinterpret_cast<const float4*>(s));
+    } else {
+        const uint2 r = __ldg(reinterpret_cast<const uint2*>(s));
+        const float2 a = __half22float2(u32_as_h2(r.x)), b = __half22float2(u32_as_h2(r.y));
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+}
+
+__device__ __forceinline__ float amax4(float4 v) {
+    return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+}
+
+// clamp(rint(x / scale)), the page quantizer's rule (kvb_pages.cu), four values packed low byte first.
+__device__ __forceinline__ uint32_t quantize4(const float4 v, float scale) {
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    uint32_t packed = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int q = min(max(__float2int_rn(__fdiv_rn(x[e], scale)), -127), 127);
+        packed |= uint32_t(q & 255) << (8 * e);
+    }
+    return packed;
+}
+
+// int8 pools. A run is the new tokens of one sequence that share a page, for one KV head of K or V: one
+// warp each. The page's scale becomes s = max(s_old, amax / 127) (s_old only if the page had rows
+// before); rows that were there are rounded again, rint(q * (s_old / s)), when the scale grew. Warps
+// look for runs among `tpw` tokens at a time: a token starts a run if it is its sequence's first new
+// one or the first of its page.
+template <typename SRC>
+__global__ void __launch_bounds__(AP_THREADS) append_i8_kernel(const AppendParams p, int tpw) {
+    const int lane = threadIdx.x & 31;
+    const int h = blockIdx.y >> 1, which = blockIdx.y & 1;
+    const long long wid = (long long)blockIdx.x * (AP_THREADS / 32) + (threadIdx.x >> 5);
+    const long long tok0 = wid * tpw;
+    pdl_wait();
+    pdl_trigger();
+    if (tok0 >= p.num_tokens) return;
+    // each of the first tpw lanes decodes one token
+    const int t = int(tok0) + lane;
+    int n = 0, at = 0;
+    long long block = -1;
+    if (lane < tpw && t < p.num_tokens) {
+        int lo = 0, hi = p.B;  // the first sequence that ends behind t
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (__ldg(p.cu_new + mid + 1) > t) hi = mid;
+            else lo = mid + 1;
+        }
+        if (lo < p.B) {
+            const int c0 = __ldg(p.cu_new + lo), c1 = min(__ldg(p.cu_new + lo + 1), p.num_tokens);
+            const int total = __ldg(p.total_lens + lo);
+            const long long start = (long long)total - (__ldg(p.cu_new + lo + 1) - c0);
+            if (c0 >= 0 && c0 <= t) {
+                if (start < 0 || (long long)total > (long long)p.max_blocks * p.page) {
+                    // -1 marks a sequence that the plan refused: it was reported there
+                    if (total != -1 && t == c0 && blockIdx.y == 0 && p.error_flag)
+                        raise_error(p.error_flag, KVB_DEVERR_LENGTH);
+                } else {
+                    const int pos = int(start) + (t - c0), pg = kvb_div(pos, p.div_page);
+                    at = pos - pg * p.page;
+                    if (t == c0 || at == 0) {
+                        const int id = __ldg(p.block_table + (size_t)lo * p.max_blocks + pg);
+                        if (id >= 0 && id < p.num_blocks) {
+                            block = id;
+                            n = min(p.page - at, c1 - t);
+                        } else if (blockIdx.y == 0 && p.error_flag) {
+                            raise_error(p.error_flag, KVB_DEVERR_BLOCK);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    const int dw = int(p.div_row.d);  // pieces of four values per row
+    const SRC* src = static_cast<const SRC*>(p.src[which]) + (long long)h * p.D;
+    const long long stride = p.stride[which];
+    for (unsigned runs = __ballot_sync(0xffffffffu, block >= 0); runs; runs &= runs - 1) {
+        const int l = __ffs(runs) - 1;
+        const int rn = __shfl_sync(0xffffffffu, n, l), rat = __shfl_sync(0xffffffffu, at, l);
+        const long long rb = __shfl_sync(0xffffffffu, block, l) * p.Hkv + h;
+        const SRC* rows = src + (tok0 + l) * stride;
+        uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<int8_t*>(p.pool[which]) + rb * p.page * p.D);
+        const int pieces = rn * dw;  // below 2^31: a page of one head is (checked by the host)
+        float amax = 0.f;
+        constexpr int U = 8;
+        for (int i0 = lane; i0 < pieces; i0 += 32 * U) {
+            float4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + 32 * u;
+                v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < pieces) {
+                    const int r = kvb_div(i, p.div_row);
+                    v[u] = load4(rows + r * stride + 4 * (i - r * dw));
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) amax = fmaxf(amax, amax4(v[u]));
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        float scale = amax / 127.0f;
+        if (rat > 0) {
+            const float old = p.scale[which][rb];
+            if (old >= scale) {
+                scale = old;
+            } else {
+                const float ratio = __fdiv_rn(old, scale);
+                for (int i = lane; i < rat * dw; i += 32) {
+                    const uint32_t x = dst[i];
+                    uint32_t y = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int q = __float2int_rn(__fmul_rn(float(int8_t(x >> (8 * e))), ratio));
+                        y |= uint32_t(q & 255) << (8 * e);
+                    }
+                    dst[i] = y;
+                }
+            }
+        }
+        __syncwarp();  // every lane has read the old scale
+        if (lane == 0) p.scale[which][rb] = scale;
+        dst += rat * dw;
+        for (int i0 = lane; i0 < pieces; i0 += 32 * U) {
+            float4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + 32 * u;
+                if (i < pieces) {
+                    const int r = kvb_div(i, p.div_row);
+                    v[u] = load4(rows + r * stride + 4 * (i - r * dw));
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + 32 * u;
+                if (i < pieces) dst[i] = scale > 0.f ? quantize4(v[u], scale) : 0u;
+            }
+        }
+    }
+}
+
+template <typename SRC, typename DST>
+cudaError_t launch_rows(const AppendParams& p, int num_sms, cudaStream_t stream) {
+    const long long pieces = (long long)p.num_tokens * p.Hkv * p.div_row.d;
+    const long long ctas = std::min<long long>((pieces + AP_THREADS - 1) / AP_THREADS, (long long)num_sms * 8);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)std::max<long long>(1, ctas), 2);
+    cfg.blockDim = dim3(AP_THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, append_rows_kernel<SRC, DST>, p);
+}
+
+template <typename SRC>
+cudaError_t launch_i8(const AppendParams& p, int num_sms, cudaStream_t stream) {
+    // tokens a warp looks at: one while that keeps the grid small, up to 32 (most are no run's first)
+    int tpw = 1;
+    while (tpw < 32 && (long long)p.num_tokens / tpw * p.Hkv * 2 > (long long)num_sms * 64) tpw *= 2;
+    const long long warps = ((long long)p.num_tokens + tpw - 1) / tpw;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((warps + AP_THREADS / 32 - 1) / (AP_THREADS / 32)), 2 * p.Hkv);
+    cfg.blockDim = dim3(AP_THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, append_i8_kernel<SRC>, p, tpw);
+}
+
+}  // namespace
+
+cudaError_t kvb_launch_step_plan(const PlanParams& p, int num_sms, cudaStream_t stream) {
+    // 1024 tokens per CTA (two per thread): enough CTAs to spread a prompt's slots, one for a decode step
+    const long long ctas = std::min<long long>(((long long)p.num_tokens + 1023) / 1024, 2ll * num_sms);
+    return kvb_launch_pdl(step_plan_kernel, (unsigned)std::max<long long>(1, ctas), PL_THREADS, 0, stream, p);
+}
+
+cudaError_t kvb_launch_append(const AppendParams& p, int src_type, int kv_type, int num_sms, cudaStream_t stream) {
+    if (kv_type == KVB_I8)
+        return src_type == KVB_F32 ? launch_i8<float>(p, num_sms, stream) : launch_i8<__half>(p, num_sms, stream);
+    if (kv_type == KVB_F32) return launch_rows<float, float>(p, num_sms, stream);
+    return src_type == KVB_F32 ? launch_rows<float, __half>(p, num_sms, stream)
+                               : launch_rows<__half, __half>(p, num_sms, stream);
+}
