@@ -69,14 +69,17 @@ int geometry(Attend& a) {
     p.Hkv = s.num_kv_heads;
     p.G = s.num_heads / s.num_kv_heads;
     p.q_scale = 1.4426950408889634f / std::sqrt(float(s.head_dim));
-    a.umma = false;
+    // (the tensor maps of fp16 pages number the pool's rows with 31 bits)
+    a.umma = a.kernel != KVB_KERNEL_SIMT &&
+             kvb_chunk_umma_supported(a.q_type, a.kv_type, a.paged, s.head_dim, p.page, p.G) &&
+             (!a.paged || a.kv_type == KVB_I8 || p.num_blocks <= 0x7fffffffll / ((long long)p.Hkv * p.page));
     if (a.kernel == KVB_KERNEL_UMMA && !a.umma)
         return invalid("the requested tensor-core kernel does not support this shape, page size or dtype");
-    p.tile_tokens = KVB_SIMT_ROWS / p.G;
-    p.unit_tokens = p.tile_tokens;
+    p.tile_tokens = (a.umma ? 128 : KVB_SIMT_ROWS) / p.G;
+    p.unit_tokens = a.umma ? 2 * p.tile_tokens : p.tile_tokens;
     p.blocks_of_new = (std::max(p.max_new, 1) + p.unit_tokens - 1) / p.unit_tokens;
     const long long base = (long long)p.blocks_of_new * p.B * p.Hkv;
-    const long long slots = 2ll * sms, least = 128;  // CTAs that run at once, keys worth a part
+    const long long slots = a.umma ? sms : 2ll * sms, least = a.umma ? 512 : 128;  // CTAs that run at once, keys worth a part
     p.splits = 1;
     if (base < slots)
         p.splits = (int)std::max<long long>(1, std::min(slots / std::max<long long>(base, 1), p.max_len / least));
@@ -85,6 +88,36 @@ int geometry(Attend& a) {
     a.workspace = 256;
     if (p.splits > 1) a.workspace += (long long)p.splits * p.T * p.H * (s.head_dim + 2) * 4 + 256;
     return KVB_OK;
+}
+
+// Tensor maps of what the tcgen05 kernel loads in tiles: fp16 queries as (dim, head, token), boxes of the
+// group's heads by a tile's tokens; fp16 pages as (dim, pool row); packed keys and values as (dim, head,
+// token). Boxes are 64 values (128 bytes) wide.
+int tensor_maps(const Attend& a, CUtensorMap* tq, CUtensorMap* tk, CUtensorMap* tv) {
+    const ChunkParams& p = a.p;
+    const unsigned long long D = (unsigned long long)a.s.head_dim;
+    std::memset(tq, 0, sizeof *tq);
+    std::memset(tk, 0, sizeof *tk);
+    std::memset(tv, 0, sizeof *tv);
+    bool ok = true;
+    auto packed = [&](CUtensorMap* m, const void* base, int heads, int64_t stride, unsigned bh, unsigned bt) {
+        const unsigned long long dims[3] = {D, (unsigned long long)heads, (unsigned long long)p.T};
+        const unsigned long long strides[2] = {2 * D, p.T > 1 ? 2ull * stride : 2 * D * heads};
+        const unsigned box[3] = {64, bh, bt};
+        ok = ok && kvb_encode_tile_map(m, base, 2, 3, dims, strides, box);
+    };
+    if (a.q_type == KVB_F16) packed(tq, p.q, p.H, p.q_stride, (unsigned)p.G, (unsigned)p.tile_tokens);
+    if (!a.paged) {
+        packed(tk, p.k, p.Hkv, p.k_stride, 1, 128);
+        packed(tv, p.v, p.Hkv, p.v_stride, 1, 128);
+    } else if (a.kv_type == KVB_F16) {
+        const unsigned long long dims[2] = {D, (unsigned long long)p.num_blocks * p.Hkv * p.page};
+        const unsigned long long strides[1] = {2 * D};
+        const unsigned box[2] = {64, (unsigned)std::min(p.page, 128)};
+        ok = ok && kvb_encode_tile_map(tk, p.k, 2, 2, dims, strides, box) &&
+             kvb_encode_tile_map(tv, p.v, 2, 2, dims, strides, box);
+    }
+    return ok ? KVB_OK : kvb_fail(KVB_ERR_DEVICE, "cuTensorMapEncodeTiled failed");
 }
 
 int run(Attend& a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -96,11 +129,18 @@ int run(Attend& a, void* workspace, size_t workspace_bytes, void* stream) {
     int sms = 0;
     if (int rc = kvb_device_sms(&sms)) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    p.next_unit = nullptr;
+    p.next_unit = a.umma && p.units > sms ? static_cast<unsigned*>(workspace) : nullptr;
     p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + 256);
     p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                         kvb_align_up(256 + sizeof(float2) * (size_t)p.splits * p.T * p.H, 256));
-    cudaError_t e = kvb_launch_chunk_simt(p, a.q_type, a.kv_type, a.s.head_dim, st);
+    cudaError_t e;
+    if (a.umma) {
+        CUtensorMap tq, tk, tv;
+        if (int rc = tensor_maps(a, &tq, &tk, &tv)) return rc;
+        e = kvb_launch_chunk_umma(p, a.q_type, a.kv_type, a.s.head_dim, &tq, &tk, &tv, sms, st);
+    } else {
+        e = kvb_launch_chunk_simt(p, a.q_type, a.kv_type, a.s.head_dim, st);
+    }
     if (e == cudaSuccess && p.splits > 1) e = kvb_launch_chunk_merge(p, a.q_type, a.s.head_dim, sms, st);
     return launched(e);
 }
