@@ -25,6 +25,7 @@ struct ChunkParams {
     unsigned* error_flag;
     float* part_o;              // splits > 1: [splits][T][H][D], each split's normalized output
     float2* part_ml;            // [splits][T][H]: (max in log2 units, sum); a NaN sum: refused
+    float* fold;                // tcgen05 kernel, long keys: each CTA's running sums [2 tiles][D / 4][128][4]
     unsigned* next_unit;        // dynamic hand-out (zeroed before the launch), or null
     long long num_blocks;
     int B, H, Hkv, G, T;
@@ -36,6 +37,10 @@ struct ChunkParams {
     long long units;            // blocks_of_new * B * splits * Hkv
     float q_scale;              // log2(e) / sqrt(D)
 };
+
+// Key tiles of 128 after which the tcgen05 kernel adds its fp32 (fp16) results' sums into `fold`.
+#define KVB_CHUNK_FOLD_F32 8
+#define KVB_CHUNK_FOLD_F16 64
 
 // Whether the tcgen05 kernel takes the call.
 bool kvb_chunk_umma_supported(int q_type, int kv_type, bool paged, int D, int page, int G);

@@ -8,13 +8,19 @@
 //     P = exp2(f S - m), l += row sums
 //     O[128 rows x D] += P V              (P in tensor memory over S, V in shared memory, MN-major)
 // with the running reference m of a row raised only when a score passes it by 2^8 (then O and l are
-// scaled in place), so O stays in tensor memory for the whole unit. One persistent CTA per SM:
+// scaled in place), so O stays in tensor memory. One persistent CTA per SM:
 //   warps 0-3, 4-7  softmax of query tiles 0 and 1, one thread per row (tensor-memory lane): while one
-//                   computes its probabilities, the products of the other run.
+//                   computes its probabilities, the products of the other run. A tile is taken in two
+//                   halves of 64 keys, and the products of the first half's probabilities start while
+//                   the second's are computed. Probabilities are computed with the reference so far and
+//                   the half's maximum beside them; only if that passes it are they computed again.
 //   warp 8          TMA producer and unit scheduler: K and V tiles into a ring of stages, Q tiles, and
 //                   the units (first blockIdx.x, then one at a time from a counter) through a small ring.
-//   warp 9          one thread issues every product.
-//   warps 10, 11    fp16 values: non-finite elements of tiles that some row does not see in full are set
+//   warp 9          one thread issues every product, the two query tiles in turn: one tile's products then
+//                   run as a block while the other tile's softmax computes. (An issuer per tile let the two
+//                   blocks mix, each took twice as long and both groups waited for both: 710 -> 797 us for
+//                   a prompt of 8192 tokens.)
+//   warp 11         fp16 values: non-finite elements of tiles that some row does not see in full are set
 //                   to 0 (0 x inf would not be 0) and, where a row does see them, added at the end.
 //   warps 12-15     int8: tiles converted to fp16 (exact), the scales are applied to the scores and to the
 //                   probabilities.
@@ -35,8 +41,13 @@ using namespace kvb_dev;
 constexpr int CU_ROWS = 128;            // query rows of a tile, keys of a tile
 constexpr int CU_SUB = CU_ROWS * 128;   // bytes of [128 rows][128 B], one 128-byte-swizzled slice
 constexpr int CU_RING = 4;              // units in flight between the roles
+constexpr int CU_POLY = 1, CU_POLY_OF = 4;  // pairs of probabilities on the FMA pipe, of so many
 constexpr int CU_CLEAN = 4;             // value tiles on their way to the cleaning warps: at most three are
 enum { SRC_F16 = 0, SRC_I8 = 1, SRC_PACKED = 2 };
+// The tensor cores add into O with truncation, an error of up to 2^-23 of O per product of 16 keys and in
+// one direction. So O is added into an fp32 sum in the workspace (rounded to nearest) and started anew
+// every so many key tiles: often for fp32 results, rarely for fp16 ones.
+constexpr int CU_FOLD_F32 = KVB_CHUNK_FOLD_F32, CU_FOLD_F16 = KVB_CHUNK_FOLD_F16;
 constexpr float CU_TAU = 8.f;    // a row's reference is raised when a score passes it by 2^CU_TAU
 constexpr float CU_SHIFT = 6.f;  // probabilities are held times 2^CU_SHIFT: below 2^14, and small ones stay normal
 
@@ -51,8 +62,8 @@ struct CCfg {
     static constexpr int FIT = (BUDGET - 2 * QTILE - NR * RAW) / ITEM;
     static constexpr int NS = FIT > 6 - NR ? 6 - NR : FIT;  // int8: at most six items in flight (scale ring)
     static constexpr int THREADS = SRC == SRC_I8 ? 512 : 384;
-    static constexpr int HELPERS = SRC == SRC_I8 ? 4 : 2;   // converting or cleaning warps
-    static constexpr int HELPER0 = SRC == SRC_I8 ? 12 : 10;
+    static constexpr int HELPERS = SRC == SRC_I8 ? 4 : 1;   // converting or cleaning warps
+    static constexpr int HELPER0 = SRC == SRC_I8 ? 12 : 11;
     // registers per thread after the split; the launch gives 65536 / THREADS, rounded down to 8
     static constexpr int REGS_LAUNCH = SRC == SRC_I8 ? 128 : 168;
     static constexpr int REGS_SOFT = SRC == SRC_I8 ? 176 : 208;
@@ -62,7 +73,7 @@ struct CCfg {
     static constexpr size_t KV_OFF = 2 * QTILE;
     static constexpr size_t RAW_OFF = KV_OFF + size_t(NS) * ITEM;
     static constexpr size_t BAR_OFF = RAW_OFF + size_t(NR) * RAW;
-    static constexpr int NBARS = 2 * NS + 2 * NR + 9 + CU_CLEAN + 2 * CU_RING;
+    static constexpr int NBARS = 2 * NS + 2 * NR + 13 + CU_CLEAN + 2 * CU_RING;
     static constexpr size_t UNIT_OFF = kvb_align_up(BAR_OFF + 8 * NBARS, 64);
     static constexpr size_t SCALE_OFF = UNIT_OFF + 64 * CU_RING;           // [4 tiles][K, V][16 pages]
     static constexpr size_t VMAX_OFF = SCALE_OFF + (NR ? 4 * 2 * 16 * 4 : 0);  // [4 tiles]
@@ -88,10 +99,56 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
+// Largest of three, NaN if one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
+}
+__device__ __forceinline__ float fmaxf_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// Two fp32 operations per instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t y;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ void unpack2(uint64_t x, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+    return y;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t y;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+
+// 2^x of a pair on the FMA pipe: x = n + r with n the nearest integer (the low bits of x + 1.5 * 2^23) and
+// r in [-1/2, 1/2], 2^r by its minimax polynomial of degree 4 (fitted to the relative error, 2.6e-6, far
+// below the fp16 rounding that follows), n added to its exponent. x is taken as at least -125.
+__device__ __forceinline__ void exp2_poly2(uint64_t x, float& a, float& b) {
+    unpack2(x, a, b);
+    x = pack2(fmaxf(a, -125.f), fmaxf(b, -125.f));
+    const uint64_t magic = pack2(12582912.f, 12582912.f), minus = pack2(-12582912.f, -12582912.f);
+    const uint64_t n = add2(x, magic);
+    const uint64_t r = fma2(add2(n, minus), pack2(-1.f, -1.f), x);
+    uint64_t y = fma2(r, pack2(0.009570102207362652f, 0.009570102207362652f), pack2(0.05591785907745361f, 0.05591785907745361f));
+    y = fma2(y, r, pack2(0.240247443318367f, 0.240247443318367f));
+    y = fma2(y, r, pack2(0.6931217908859253f, 0.6931217908859253f));
+    y = fma2(y, r, pack2(0.9999992847442627f, 0.9999992847442627f));
+    float na, nb;
+    unpack2(n, na, nb);
+    unpack2(y, a, b);
+    a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(na) << 23));
+    b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(nb) << 23));
 }
 
 // Pins the loaded values behind the wait that makes them valid.
@@ -120,8 +177,9 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
     uint64_t* q_full = raw_empty + C::NR;  // [2] query tile in shared memory
     uint64_t* q_empty = q_full + 2;      // both query tiles' score products are done
     uint64_t* s_full = q_empty + 1;      // [2] scores ready, and every product before them done
-    uint64_t* p_full = s_full + 2;       // [2] probabilities written, O scaled
-    uint64_t* o_full = p_full + 2;       // [2] the unit's O complete
+    uint64_t* p_full = s_full + 2;       // [2][2 halves] probabilities written, O scaled
+    uint64_t* half_done = p_full + 4;    // [2] the products of the first half done
+    uint64_t* o_full = half_done + 2;    // [2] the unit's O complete
     uint64_t* dirty_full = o_full + 2;   // [CU_CLEAN] a value tile loaded that passes the cleaning warps first
     uint64_t* r_full = dirty_full + CU_CLEAN;  // [CU_RING] unit published
     uint64_t* r_empty = r_full + CU_RING;
@@ -139,7 +197,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             if (b < empty) n = SRC == SRC_I8 ? C::HELPERS : 1;
             else if (b >= raw_empty && b < q_full) n = C::HELPERS;
             else if (b >= q_full && b < q_empty) n = QF32 ? 4 : 1;
-            else if (b >= p_full && b < o_full) n = 4;
+            else if (b >= p_full && b < half_done) n = 4;
             else if (b >= r_empty) n = 1 + 8 + C::HELPERS;  // product issuer, softmax warps, helpers
             mbar_init(b, n);
         }
@@ -173,6 +231,8 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
         const int lp = SRC == SRC_I8 ? __ffs(p.page) - 1 : 0;
         uint32_t ns = 0, no = 0;  // score tiles and units that this group has taken
         uint32_t tiles = 0;       // key tiles of the CTA so far (int8 scale ring)
+        constexpr int FOLD = QF32 ? CU_FOLD_F32 : CU_FOLD_F16;
+        float4* fold = reinterpret_cast<float4*>(p.fold) + (size_t)(2 * blockIdx.x + t) * (D / 4) * 128 + r;
         for (int e = 0;; ++e) {
             wait(&r_full[e % CU_RING], e / CU_RING);
             const RingUnit& R = ring(e);
@@ -239,105 +299,173 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             float ref = -INFINITY;  // probabilities are 2^(f s - ref)
             float l = 0.f;
             float vexp = 0.f;       // int8: 2^-e, probabilities times the value scales times this; 0: not set
+            float older = 1.f;      // what the folded sum has to be scaled by
+            int folds = 0;
+            // O (complete up to here) and the folded sum times `scale`
+            auto rescale = [&](float scale) {
+                older *= scale;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    tc_ld32(to + c, o);
+                    tc_wait_ld();
+                    pin<32>(o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * scale);
+                    tc_st32(to + c, o);
+                }
+            };
             for (int j = 0; j < nt; ++j) {
                 wait(&s_full[t], ns);
-                ++ns;
                 if (stop()) break;
                 tc_fence_after();
-                uint32_t s[128];
-                tc_ld32(ts, s);
-                tc_ld32(ts + 32, s + 32);
-                tc_ld32(ts + 64, s + 64);
-                tc_ld32(ts + 96, s + 96);
-                tc_wait_ld();
-                pin<128>(s);
                 const int k0 = (kt0 + j) * CU_ROWS;
                 const bool masked = k0 + CU_ROWS > all_see;
                 const float* scales = s_scale + ((tiles + j) & 3) * 32;
-                if constexpr (SRC == SRC_I8) {
+                if (j > 0 && j % FOLD == 0) {
+                    // the products of the tiles before are done, the next one starts O anew
+                    const bool plain = __all_sync(0xffffffffu, older == 1.f);
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tc_ld32(to + c, o);
+                        tc_wait_ld();
+                        pin<32>(o);
+                        float4* at = fold + (c / 4) * 128;
 #pragma unroll
-                    for (int c = 0; c < 128; c += 8) {
-                        const float ks = scales[c >> lp];  // (pages of 128 tokens or more: one)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) s[c + i] = __float_as_uint(__uint_as_float(s[c + i]) * ks);
+                        for (int i = 0; i < 8; ++i, at += 128) {
+                            float4 x = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                   __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                            if (folds == 0) {
+                                __stcg(at, x);
+                            } else if (plain) {
+                                asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(x.x), "f"(x.y),
+                                             "f"(x.z), "f"(x.w)
+                                             : "memory");
+                            } else {
+                                const float4 y = __ldcg(at);
+                                x.x = fmaf(y.x, older, x.x), x.y = fmaf(y.y, older, x.y);
+                                x.z = fmaf(y.z, older, x.z), x.w = fmaf(y.w, older, x.w);
+                                __stcg(at, x);
+                            }
+                        }
                     }
-                }
-                if (masked) {
-                    const int lim = limit - k0;
-#pragma unroll
-                    for (int c = 0; c < 128; ++c)
-                        if (c >= lim) s[c] = 0xff800000u;  // -inf
-                }
-                float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < 128; c += 4) {
-                    m0 = max3(m0, __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-                    m1 = max3(m1, __uint_as_float(s[c + 2]), __uint_as_float(s[c + 3]));
-                }
-                const float mt = fmaxf(m0, m1) * f - CU_SHIFT;
-                // a new reference: O and l follow
-                float scale = 1.f;
-                bool move = mt > ref + CU_TAU;
-                if (move) {
-                    scale = ref == -INFINITY ? 0.f : ex2(ref - mt);
-                    ref = mt;
-                    l *= scale;
+                    ++folds;
+                    older = 1.f;
                 }
                 if constexpr (SRC == SRC_I8) {
                     const float vm = s_vmax[(tiles + j) & 3];  // the tile's largest finite value scale
                     if (vexp == 0.f || vm * vexp > 2.f) {      // (the same in every row)
                         const int x = min(max(int(__float_as_uint(vm) >> 23) - 127, -100), 125);
                         const float ve = __uint_as_float(uint32_t(126 - x) << 23);  // vm * ve in [0.5, 1)
-                        if (vexp != 0.f) {
-                            scale *= ve / vexp;
-                            move = true;
-                        }
+                        if (vexp != 0.f) rescale(ve / vexp);
                         vexp = ve;
                     }
                 }
-                if (j > 0 && __any_sync(0xffffffffu, move)) {
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t s[64];
+                    tc_ld32(ts + 64 * half, s);
+                    tc_ld32(ts + 64 * half + 32, s + 32);
+                    tc_wait_ld();
+                    pin<64>(s);
+                    const int kh = k0 + 64 * half;
+                    if constexpr (SRC == SRC_I8) {
 #pragma unroll
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t o[32];
-                        tc_ld32(to + c, o);
-                        tc_wait_ld();
-                        pin<32>(o);
+                        for (int c = 0; c < 64; c += 8) {
+                            const float ks = scales[(64 * half + c) >> lp];  // (pages of 128 tokens or more: one)
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * scale);
-                        tc_st32(to + c, o);
-                    }
-                }
-                const float base = ref == -INFINITY ? 0.f : -ref;
-                float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-                for (int c0 = 0; c0 < 128; c0 += 32) {
-                    uint32_t hi[QF32 ? 32 : 16];
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        float a = ex2(fmaf(__uint_as_float(s[c0 + i]), f, base));
-                        float b = ex2(fmaf(__uint_as_float(s[c0 + i + 1]), f, base));
-                        l0 += a;
-                        l1 += b;
-                        if constexpr (SRC == SRC_I8) {
-                            const float vs = scales[16 + ((c0 + i) >> lp)] * vexp;
-                            a = a * vs;
-                            b = b * vs;
-                            if (masked) {  // the scale of a page that this row does not see may be anything
-                                if (k0 + c0 + i >= limit) a = 0.f;
-                                if (k0 + c0 + i + 1 >= limit) b = 0.f;
-                            }
+                            for (int i = 0; i < 8; ++i) s[c + i] = __float_as_uint(__uint_as_float(s[c + i]) * ks);
                         }
-                        if constexpr (QF32) split_hi_lo(a, b, hi[i / 2], hi[16 + i / 2]);
-                        else hi[i / 2] = h2_as_u32(__floats2half2_rn(a, b));
                     }
-                    if constexpr (QF32) tc_st32(ts + c0, hi);       // hi, lo of 32 keys: 16 columns each
-                    else tc_st16(ts + c0 / 2, hi);
+                    if (masked) {
+                        const int lim = limit - kh;
+#pragma unroll
+                        for (int c = 0; c < 64; ++c)
+                            if (c >= lim) s[c] = 0xff800000u;  // -inf
+                    }
+                    uint32_t pr[QF32 ? 64 : 32];
+                    float sum, mt;
+                    auto probabilities = [&](float base) {
+                        const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
+                        uint64_t l0 = 0, l1 = 0;
+                        float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < 64; i += 2) {
+                            const float s0 = __uint_as_float(s[i]), s1 = __uint_as_float(s[i + 1]);
+                            if (i & 2) m1 = max3_nan(m1, s0, s1);
+                            else m0 = max3_nan(m0, s0, s1);
+                            const uint64_t x = fma2(pack2(s0, s1), f2, b2);
+                            float a, b;
+                            if (!QF32 && (i / 2) % CU_POLY_OF < CU_POLY) {
+                                exp2_poly2(x, a, b);
+                            } else {
+                                unpack2(x, a, b);
+                                a = ex2(a);
+                                b = ex2(b);
+                            }
+                            if (i & 2) l1 = add2(l1, pack2(a, b));
+                            else l0 = add2(l0, pack2(a, b));
+                            if constexpr (SRC == SRC_I8) {
+                                const float vs = scales[16 + ((64 * half + i) >> lp)] * vexp;
+                                a *= vs;
+                                b *= vs;
+                                if (masked) {  // the scale of a page that this row does not see may be anything
+                                    if (kh + i >= limit) a = 0.f;
+                                    if (kh + i + 1 >= limit) b = 0.f;
+                                }
+                            }
+                            if constexpr (QF32) split_hi_lo(a, b, pr[32 * (i / 32) + i % 32 / 2], pr[32 * (i / 32) + 16 + i % 32 / 2]);
+                            else pr[i / 2] = h2_as_u32(__floats2half2_rn(a, b));
+                        }
+                        float a, b;
+                        unpack2(add2(l0, l1), a, b);
+                        sum = a + b;
+                        mt = fmaxf_nan(m0, m1);
+                    };
+                    bool move = j == 0 && half == 0;
+                    if (!move) {
+                        probabilities(ref == -INFINITY ? 0.f : -ref);
+                        move = mt * f - CU_SHIFT > ref + CU_TAU;
+                    } else {
+                        float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < 64; i += 4) {
+                            m0 = max3_nan(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                            m1 = max3_nan(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+                        }
+                        mt = fmaxf_nan(m0, m1);
+                    }
+                    if (__any_sync(0xffffffffu, move)) {
+                        // a new reference where a score passed the old one: O, l and these probabilities follow
+                        float scale = 1.f;
+                        const float top = mt * f - CU_SHIFT;
+                        if (top > ref) {
+                            scale = ref == -INFINITY ? 0.f : ex2(ref - top);
+                            ref = top;
+                            l *= scale;
+                        }
+                        if (j > 0 || half) {
+                            if (half) wait(&half_done[t], ns);
+                            tc_fence_after();
+                            rescale(scale);
+                        }
+                        probabilities(ref == -INFINITY ? 0.f : -ref);
+                    }
+                    // a NaN or +inf score makes the whole row NaN
+                    l += mt < INFINITY ? sum : __int_as_float(0x7fc00000);
+                    if constexpr (QF32) {  // hi, lo of 32 keys: 16 columns each
+                        tc_st32(ts + 64 * half, pr);
+                        tc_st32(ts + 64 * half + 32, pr + 32);
+                    } else {
+                        tc_st32(ts + 32 * half, pr);
+                    }
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * t + half]);
                 }
-                l += l0 + l1;
-                tc_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[t]);
+                ++ns;
             }
             tiles += nall;
             if (nt > 0) {
@@ -365,6 +493,16 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = 0;
+                }
+                if (folds > 0) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float4 x = __ldcg(fold + (c / 4 + i) * 128);
+                        o[4 * i] = __float_as_uint(fmaf(x.x, older, __uint_as_float(o[4 * i])));
+                        o[4 * i + 1] = __float_as_uint(fmaf(x.y, older, __uint_as_float(o[4 * i + 1])));
+                        o[4 * i + 2] = __float_as_uint(fmaf(x.z, older, __uint_as_float(o[4 * i + 2])));
+                        o[4 * i + 3] = __float_as_uint(fmaf(x.w, older, __uint_as_float(o[4 * i + 3])));
+                    }
                 }
                 if (SRC != SRC_I8 && odd && !bad && live) {
                     const int first = max(kt0, all_see / CU_ROWS) * CU_ROWS;
@@ -557,8 +695,39 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             if (lane == 0) {
                 constexpr uint32_t id_s = instr_desc(1, 0, 0, 0, 0, 128, 128);
                 constexpr uint32_t id_o = instr_desc(1, 0, 0, 0, 1, D, 128);
-                uint32_t item = 0;
-                uint32_t nq[2] = {0, 0}, np[2] = {0, 0};
+                constexpr int FOLD = QF32 ? CU_FOLD_F32 : CU_FOLD_F16;
+                // descriptors of the first stage; a byte offset of o adds o / 16
+                const uint64_t kd = smem_desc(sbase + uint32_t(C::KV_OFF), 16, 1024);
+                const uint64_t vd = smem_desc(sbase + uint32_t(C::KV_OFF), CU_SUB, 1024);
+                const uint64_t qd = smem_desc(sbase + uint32_t(C::Q_OFF), 16, 1024);
+                uint32_t item = 0, nq0 = 0, nq1 = 0, np0 = 0, np1 = 0;
+                auto scores = [&](int t, uint32_t it) {
+                    const uint64_t k = kd + (it % NS) * (C::ITEM / 16), q = qd + t * (C::QTILE / 16);
+#pragma unroll
+                    for (int part = 0; part < (QF32 ? 2 : 1); ++part)
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) {
+                            const uint32_t off = ((i / 4) * CU_SUB + (i % 4) * 32) / 16;
+                            tc_mma<1>(tmem + 128 * t, q + (part * NSUB * CU_SUB / 16 + off), k + off, id_s, part > 0 || i > 0);
+                        }
+                    tc_commit(&s_full[t]);
+                };
+                auto values = [&](int t, uint32_t it, int half, bool keep) {
+                    const uint64_t v = vd + (it % NS) * (C::ITEM / 16) + half * (64 * 128 / 16);
+                    const uint32_t ts = tmem + 128 * t + (QF32 ? 64 : 32) * half, to = tmem + 256 + D * t;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint64_t b = v + i * (2048 / 16);
+                        if constexpr (QF32) {
+                            const uint32_t a = ts + 32 * (i / 2) + 8 * (i % 2);
+                            tc_mma_ts(to, a, b, id_o, keep || i > 0);
+                            tc_mma_ts(to, a + 16, b, id_o, 1);
+                        } else {
+                            tc_mma_ts(to, ts + 8 * i, b, id_o, keep || i > 0);
+                        }
+                    }
+                };
+                auto ready = [&](uint32_t it) { wait(&full[it % NS], it / NS); };
                 for (int e = 0; !*s_abort; ++e) {
                     wait(&r_full[e % CU_RING], e / CU_RING);
                     const RingUnit& R = ring(e);
@@ -567,75 +736,52 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     if (state < 0) break;
                     const int nj = max(nt0, nt1);
                     if (nj == 0) continue;
-                    const uint32_t k_item = item;  // K of tile j is item k_item + 2 j, V the next one
-                    auto scores = [&](int t, int j) {
-                        const uint32_t kt = sbase + uint32_t(C::KV_OFF) + ((k_item + 2 * j) % NS) * C::ITEM;
-                        const uint32_t qt = sbase + uint32_t(C::Q_OFF) + t * C::QTILE;
-#pragma unroll
-                        for (int part = 0; part < (QF32 ? 2 : 1); ++part)
-#pragma unroll
-                            for (int i = 0; i < D / 16; ++i) {
-                                const uint32_t off = (i / 4) * CU_SUB + (i % 4) * 32;
-                                tc_mma<1>(tmem + 128 * t, smem_desc(qt + part * NSUB * CU_SUB + off, 16, 1024),
-                                          smem_desc(kt + off, 16, 1024), id_s, part > 0 || i > 0);
-                            }
-                        tc_commit(&s_full[t]);
-                    };
-                    auto values = [&](int t, int j) {
-                        const uint32_t vt = sbase + uint32_t(C::KV_OFF) + ((k_item + 2 * j + 1) % NS) * C::ITEM;
-#pragma unroll
-                        for (int i = 0; i < CU_ROWS / 16; ++i) {
-                            const uint64_t b = smem_desc(vt + i * 2048, CU_SUB, 1024);
-                            if constexpr (QF32) {
-                                const uint32_t a = tmem + 128 * t + 32 * (i / 2) + 8 * (i % 2);
-                                tc_mma_ts(tmem + 256 + D * t, a, b, id_o, j > 0 || i > 0);
-                                tc_mma_ts(tmem + 256 + D * t, a + 16, b, id_o, 1);
-                            } else {
-                                tc_mma_ts(tmem + 256 + D * t, tmem + 128 * t + 8 * i, b, id_o, j > 0 || i > 0);
-                            }
-                        }
-                    };
-                    auto ready = [&](uint32_t it) { wait(&full[it % NS], it / NS); };
-                    auto first = [&](int t) {
-                        wait(&q_full[t], nq[t]);
-                        ++nq[t];
+                    // K of key tile j is item `item` + 2 j, its V the next one
+                    ready(item);
+                    if (nt0 > 0) {
+                        wait(&q_full[0], nq0++);
                         tc_fence_after();
-                        scores(t, 0);
-                    };
-                    ready(k_item);
-                    if (nt0 > 0) first(0);
-                    if (nt1 > 0) first(1);
-                    tc_commit(&empty[k_item % NS]);
+                        scores(0, item);
+                    }
+                    if (nt1 > 0) {
+                        wait(&q_full[1], nq1++);
+                        tc_fence_after();
+                        scores(1, item);
+                    }
+                    tc_commit(&empty[item % NS]);
                     if (nj == 1) tc_commit(q_empty);
                     for (int j = 0; j < nj && !*s_abort; ++j) {
-                        const bool more = j + 1 < nj;
-                        ready(k_item + 2 * j + 1);
-                        bool next_k = false;
+                        const uint32_t iv = item + 1, ik = item + 2;
+                        bool have_k = false;
+                        ready(iv);
 #pragma unroll
                         for (int t = 0; t < 2; ++t) {
                             const int nt = t ? nt1 : nt0;
                             if (j >= nt) continue;
-                            wait(&p_full[t], np[t]);
-                            ++np[t];
-                            if (*s_abort) break;
+                            uint32_t& np = t ? np1 : np0;
+                            wait(&p_full[2 * t], np);
                             tc_fence_after();
-                            values(t, j);
+                            values(t, iv, 0, j % FOLD != 0);
+                            tc_commit(&half_done[t]);
+                            wait(&p_full[2 * t + 1], np);
+                            tc_fence_after();
+                            values(t, iv, 1, true);
+                            ++np;
+                            if (*s_abort) break;
                             if (j + 1 < nt) {
-                                if (!next_k) {
-                                    ready(k_item + 2 * j + 2);
-                                    tc_fence_after();
-                                    next_k = true;
-                                }
-                                scores(t, j + 1);
+                                if (!have_k) ready(ik);
+                                have_k = true;
+                                tc_fence_after();
+                                scores(t, ik);
                             } else {
                                 tc_commit(&o_full[t]);
                             }
                         }
-                        tc_commit(&empty[(k_item + 2 * j + 1) % NS]);
-                        if (more) tc_commit(&empty[(k_item + 2 * j + 2) % NS]);
+                        tc_commit(&empty[iv % NS]);
+                        if (j + 1 < nj) tc_commit(&empty[ik % NS]);
                         if (j + 2 == nj) tc_commit(q_empty);
+                        item += 2;
                     }
-                    item += 2 * nj;
                 }
             }
         } else if (warp >= C::HELPER0) {

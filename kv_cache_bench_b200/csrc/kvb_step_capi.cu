@@ -39,7 +39,7 @@ struct Attend {
     int q_type, kv_type, kernel;
     bool paged;
     ChunkParams p;
-    int64_t workspace;
+    int64_t workspace, fold_off;
     bool umma;
 };
 
@@ -87,6 +87,11 @@ int geometry(Attend& a) {
     if (p.units >= (1ll << 31)) return invalid("more than 2^31 work units");
     a.workspace = 256;
     if (p.splits > 1) a.workspace += (long long)p.splits * p.T * p.H * (s.head_dim + 2) * 4 + 256;
+    a.workspace = (int64_t)kvb_align_up((size_t)a.workspace, 256);
+    a.fold_off = a.workspace;
+    const int fold = a.q_type == KVB_F32 ? KVB_CHUNK_FOLD_F32 : KVB_CHUNK_FOLD_F16;
+    if (a.umma && p.max_len > fold * 128)
+        a.workspace += std::min<long long>(p.units, sms) * 2 * 128 * s.head_dim * 4;
     return KVB_OK;
 }
 
@@ -133,6 +138,7 @@ int run(Attend& a, void* workspace, size_t workspace_bytes, void* stream) {
     p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + 256);
     p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                         kvb_align_up(256 + sizeof(float2) * (size_t)p.splits * p.T * p.H, 256));
+    p.fold = reinterpret_cast<float*>(static_cast<char*>(workspace) + a.fold_off);
     cudaError_t e;
     if (a.umma) {
         CUtensorMap tq, tk, tv;
