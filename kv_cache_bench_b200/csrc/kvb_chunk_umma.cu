@@ -215,8 +215,12 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
     pdl_wait();
     pdl_trigger();
 
+    // False once a wait has given up (here, or elsewhere in the CTA where this one would block).
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (!*s_abort && !mbar_wait_bounded(bar, parity & 1, s_abort)) *s_abort = 1;
+        if (mbar_try_wait(bar, parity & 1)) return true;
+        if (!*s_abort && mbar_wait_bounded(bar, parity & 1, s_abort)) return true;
+        *s_abort = 1;
+        return false;
     };
     auto stop = [&]() { return __any_sync(0xffffffffu, *s_abort) != 0; };  // the same answer in a whole warp
 
@@ -316,8 +320,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 }
             };
             for (int j = 0; j < nt; ++j) {
-                wait(&s_full[t], ns);
-                if (stop()) break;
+                if (__any_sync(0xffffffffu, !wait(&s_full[t], ns))) break;
                 tc_fence_after();
                 const int k0 = (kt0 + j) * CU_ROWS;
                 const bool masked = k0 + CU_ROWS > all_see;
@@ -692,7 +695,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             publish(end, make_int2(0, 0), 0, 0);
         } else if (warp == 9) {
             // ------------------------------------------------------------ products
-            if (lane == 0) {
+            if (tc_elect()) {
                 constexpr uint32_t id_s = instr_desc(1, 0, 0, 0, 0, 128, 128);
                 constexpr uint32_t id_o = instr_desc(1, 0, 0, 0, 1, D, 128);
                 constexpr int FOLD = QF32 ? CU_FOLD_F32 : CU_FOLD_F16;
@@ -727,7 +730,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                         }
                     }
                 };
-                auto ready = [&](uint32_t it) { wait(&full[it % NS], it / NS); };
+                auto ready = [&](uint32_t it) { return wait(&full[it % NS], it / NS); };
                 for (int e = 0; !*s_abort; ++e) {
                     wait(&r_full[e % CU_RING], e / CU_RING);
                     const RingUnit& R = ring(e);
@@ -759,19 +762,16 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                             const int nt = t ? nt1 : nt0;
                             if (j >= nt) continue;
                             uint32_t& np = t ? np1 : np0;
-                            wait(&p_full[2 * t], np);
+                            if (!wait(&p_full[2 * t], np)) break;
                             tc_fence_after();
                             values(t, iv, 0, j % FOLD != 0);
                             tc_commit(&half_done[t]);
-                            wait(&p_full[2 * t + 1], np);
+                            if (j + 1 < nt && !have_k) have_k = ready(ik);  // while the second half is computed
+                            if (!wait(&p_full[2 * t + 1], np)) break;
                             tc_fence_after();
                             values(t, iv, 1, true);
                             ++np;
-                            if (*s_abort) break;
                             if (j + 1 < nt) {
-                                if (!have_k) ready(ik);
-                                have_k = true;
-                                tc_fence_after();
                                 scores(t, ik);
                             } else {
                                 tc_commit(&o_full[t]);
