@@ -9,20 +9,23 @@
 //     O[128 rows x D] += P V              (P in tensor memory over S, V in shared memory, MN-major)
 // with the running reference m of a row raised only when a score passes it by 2^8 (then O and l are
 // scaled in place), so O stays in tensor memory. One persistent CTA per SM:
-//   warps 0-3, 4-7  softmax of query tiles 0 and 1, one thread per row (tensor-memory lane): while one
-//                   computes its probabilities, the products of the other run. A tile is taken in two
-//                   halves of 64 keys, and the products of the first half's probabilities start while
-//                   the second's are computed. Probabilities are computed with the reference so far and
-//                   the half's maximum beside them; only if that passes it are they computed again.
-//   warp 8          TMA producer and unit scheduler: K and V tiles into a ring of stages, Q tiles, and
+//   warps 0-15      softmax: eight warps per query tile, a thread per row (tensor-memory lane) and half of
+//                   the key tile. While one tile's warps compute, the products of the other run; four
+//                   compute warps per scheduler hide each other's latencies (with two, a key tile took
+//                   2700 cycles of softmax instead of about 1400, the same instructions). Probabilities are
+//                   computed with the reference so far and the maximum beside them; only if a score passes
+//                   the reference are they computed again.
+//   warp 16         TMA producer and unit scheduler: K and V tiles into a ring of stages, Q tiles, and
 //                   the units (first blockIdx.x, then one at a time from a counter) through a small ring.
-//   warp 9          one thread issues every product, the two query tiles in turn: one tile's products then
-//                   run as a block while the other tile's softmax computes. (An issuer per tile let the two
-//                   blocks mix, each took twice as long and both groups waited for both: 710 -> 797 us for
-//                   a prompt of 8192 tokens.)
-//   warp 11         fp16 values: non-finite elements of tiles that some row does not see in full are set
+//   warps 17, 18    one elected thread each issues the score products and the value products. (A lane
+//                   chosen by its number instead of elect.sync took 85 cycles a product, longer than the
+//                   product, and one thread for both kinds was the bottleneck: with its share of waits and
+//                   commits it took 2000 cycles a key tile and query tile, twice the products' time.) With
+//                   split operands (QF32) a tile's scores and probabilities share their columns, and one
+//                   thread issues both kinds in order.
+//   warp 19         fp16 values: non-finite elements of tiles that some row does not see in full are set
 //                   to 0 (0 x inf would not be 0) and, where a row does see them, added at the end.
-//   warps 12-15     int8: tiles converted to fp16 (exact), the scales are applied to the scores and to the
+//   warps 20-23     int8: tiles converted to fp16 (exact), the scales are applied to the scores and to the
 //                   probabilities.
 // fp32 queries (QF32) keep fp32-level results: q and p are split as fp16(x) + fp16(x - fp16(x)) (about 22
 // bits; q prescaled per row by a power of two) and both products run on both halves.
@@ -40,16 +43,16 @@ using namespace kvb_dev;
 
 constexpr int CU_ROWS = 128;            // query rows of a tile, keys of a tile
 constexpr int CU_SUB = CU_ROWS * 128;   // bytes of [128 rows][128 B], one 128-byte-swizzled slice
-constexpr int CU_RING = 4;              // units in flight between the roles
-constexpr int CU_POLY = 1, CU_POLY_OF = 4;  // pairs of probabilities on the FMA pipe, of so many
+constexpr int CU_RING = 2;              // units in flight between the roles
+constexpr int CU_POLY = 0, CU_POLY_OF = 4;  // pairs of probabilities on the FMA pipe, of so many
 constexpr int CU_CLEAN = 4;             // value tiles on their way to the cleaning warps: at most three are
 enum { SRC_F16 = 0, SRC_I8 = 1, SRC_PACKED = 2 };
 // The tensor cores add into O with truncation, an error of up to 2^-23 of O per product of 16 keys and in
 // one direction. So O is added into an fp32 sum in the workspace (rounded to nearest) and started anew
 // every so many key tiles: often for fp32 results, rarely for fp16 ones.
 constexpr int CU_FOLD_F32 = KVB_CHUNK_FOLD_F32, CU_FOLD_F16 = KVB_CHUNK_FOLD_F16;
-constexpr float CU_TAU = 8.f;    // a row's reference is raised when a score passes it by 2^CU_TAU
-constexpr float CU_SHIFT = 6.f;  // probabilities are held times 2^CU_SHIFT: below 2^14, and small ones stay normal
+constexpr float CU_SHIFT = 5.f;  // a row's highest score so far has probability 2^CU_SHIFT: small ones stay normal in fp16
+constexpr float CU_MOST = 16384.f;  // a key tile's probabilities of a row may sum to this before the reference moves
 
 template <int SRC, bool QF32, int D>
 struct CCfg {
@@ -61,23 +64,30 @@ struct CCfg {
     static constexpr int NR = SRC == SRC_I8 ? (QF32 ? 2 : 3) : 0;
     static constexpr int FIT = (BUDGET - 2 * QTILE - NR * RAW) / ITEM;
     static constexpr int NS = FIT > 6 - NR ? 6 - NR : FIT;  // int8: at most six items in flight (scale ring)
-    static constexpr int THREADS = SRC == SRC_I8 ? 512 : 384;
+    static constexpr int SOFT = 8;                          // softmax warps
     static constexpr int HELPERS = SRC == SRC_I8 ? 4 : 1;   // converting or cleaning warps
-    static constexpr int HELPER0 = SRC == SRC_I8 ? 12 : 11;
+    static constexpr int HELPER0 = SOFT + (SRC == SRC_I8 ? 4 : 3);
+    static constexpr int THREADS = 32 * (SOFT + (SRC == SRC_I8 ? 8 : 4));
     // registers per thread after the split; the launch gives 65536 / THREADS, rounded down to 8
-    static constexpr int REGS_LAUNCH = SRC == SRC_I8 ? 128 : 168;
-    static constexpr int REGS_SOFT = SRC == SRC_I8 ? 176 : 208;
+    static constexpr int REGS_LAUNCH = 65536 / THREADS / 8 * 8;
     static constexpr int REGS_REST = SRC == SRC_I8 ? 80 : 88;
-    static_assert(256 * REGS_SOFT + (THREADS - 256) * REGS_REST <= THREADS * REGS_LAUNCH, "register split");
+    static constexpr int REGS_SOFT = (THREADS * REGS_LAUNCH - (THREADS - 32 * SOFT) * REGS_REST) / (32 * SOFT) / 8 * 8;
+    // Tensor-memory columns. fp16 probabilities have their own, so that a tile's next scores need not wait
+    // for its value product; split ones lie over their scores. O of tile t is at O_COL + D t.
+    static constexpr bool ALIAS = QF32;
+    static constexpr int SBUFS = ALIAS || D == 64 ? 2 : 1;    // score buffers: the tiles', or one that they share
+    static constexpr int O_COL = ALIAS ? 256 : 128 * SBUFS + 128;
+    static_assert(O_COL + 2 * D <= 512, "tensor memory");
+    static constexpr int SR = ALIAS ? 4 : 8;                  // int8: key tiles whose scales are kept
     static constexpr size_t Q_OFF = 0;
     static constexpr size_t KV_OFF = 2 * QTILE;
     static constexpr size_t RAW_OFF = KV_OFF + size_t(NS) * ITEM;
     static constexpr size_t BAR_OFF = RAW_OFF + size_t(NR) * RAW;
-    static constexpr int NBARS = 2 * NS + 2 * NR + 13 + CU_CLEAN + 2 * CU_RING;
+    static constexpr int NBARS = 2 * NS + 2 * NR + 11 + CU_CLEAN + 2 * CU_RING;
     static constexpr size_t UNIT_OFF = kvb_align_up(BAR_OFF + 8 * NBARS, 64);
-    static constexpr size_t SCALE_OFF = UNIT_OFF + 64 * CU_RING;           // [4 tiles][K, V][16 pages]
-    static constexpr size_t VMAX_OFF = SCALE_OFF + (NR ? 4 * 2 * 16 * 4 : 0);  // [4 tiles]
-    static constexpr size_t MISC_OFF = kvb_align_up(VMAX_OFF + 16, 16);
+    static constexpr size_t SCALE_OFF = UNIT_OFF + 64 * CU_RING;           // [SR tiles][K, V][16 pages]
+    static constexpr size_t VMAX_OFF = SCALE_OFF + (NR ? SR * 2 * 16 * 4 : 0);  // [SR tiles]
+    static constexpr size_t MISC_OFF = kvb_align_up(VMAX_OFF + (NR ? SR * 4 : 0), 16);
     static constexpr size_t SMEM = MISC_OFF + 16 + 1024;
     static_assert(NS >= 2 && SMEM <= 227 * 1024, "shared memory budget");
     static_assert(KV_OFF % 1024 == 0 && RAW_OFF % 1024 == 0, "swizzled tiles need 1024-byte alignment");
@@ -125,19 +135,25 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
     return y;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t y;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t y;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
     return y;
 }
 
-// 2^x of a pair on the FMA pipe: x = n + r with n the nearest integer (the low bits of x + 1.5 * 2^23) and
-// r in [-1/2, 1/2], 2^r by its minimax polynomial of degree 4 (fitted to the relative error, 2.6e-6, far
-// below the fp16 rounding that follows), n added to its exponent. x is taken as at least -125.
+// 2^x of a pair on the FMA pipe: x = n + r with n the nearest integer and r in [-1/2, 1/2], 2^r by its
+// minimax polynomial of degree 4 (fitted to the relative error, 2.6e-6, far below the fp16 rounding that
+// follows), times 2^n. x + 1.5 * 2^23 + 127 holds n + 127, 2^n's exponent, in its low bits. x is taken as at
+// least -126; NaN stays NaN.
 __device__ __forceinline__ void exp2_poly2(uint64_t x, float& a, float& b) {
     unpack2(x, a, b);
-    x = pack2(fmaxf(a, -125.f), fmaxf(b, -125.f));
-    const uint64_t magic = pack2(12582912.f, 12582912.f), minus = pack2(-12582912.f, -12582912.f);
+    x = pack2(fmaxf_nan(a, -126.f), fmaxf_nan(b, -126.f));
+    const uint64_t magic = pack2(12583039.f, 12583039.f), minus = pack2(-12583039.f, -12583039.f);
     const uint64_t n = add2(x, magic);
     const uint64_t r = fma2(add2(n, minus), pack2(-1.f, -1.f), x);
     uint64_t y = fma2(r, pack2(0.009570102207362652f, 0.009570102207362652f), pack2(0.05591785907745361f, 0.05591785907745361f));
@@ -146,9 +162,8 @@ __device__ __forceinline__ void exp2_poly2(uint64_t x, float& a, float& b) {
     y = fma2(y, r, pack2(0.9999992847442627f, 0.9999992847442627f));
     float na, nb;
     unpack2(n, na, nb);
+    y = mul2(y, pack2(__uint_as_float(__float_as_uint(na) << 23), __uint_as_float(__float_as_uint(nb) << 23)));
     unpack2(y, a, b);
-    a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(na) << 23));
-    b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(nb) << 23));
 }
 
 // Pins the loaded values behind the wait that makes them valid.
@@ -176,11 +191,11 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
     uint64_t* raw_empty = raw_full + C::NR;
     uint64_t* q_full = raw_empty + C::NR;  // [2] query tile in shared memory
     uint64_t* q_empty = q_full + 2;      // both query tiles' score products are done
-    uint64_t* s_full = q_empty + 1;      // [2] scores ready, and every product before them done
-    uint64_t* p_full = s_full + 2;       // [2][2 halves] probabilities written, O scaled
-    uint64_t* half_done = p_full + 4;    // [2] the products of the first half done
-    uint64_t* o_full = half_done + 2;    // [2] the unit's O complete
-    uint64_t* dirty_full = o_full + 2;   // [CU_CLEAN] a value tile loaded that passes the cleaning warps first
+    uint64_t* s_full = q_empty + 1;      // [2] scores of the tile ready
+    uint64_t* s_free = s_full + 2;       // [SBUFS] scores read into registers (not with ALIAS)
+    uint64_t* p_full = s_free + 2;       // [2] probabilities written, O scaled
+    uint64_t* pv_done = p_full + 2;      // [2] a value product done
+    uint64_t* dirty_full = pv_done + 2;   // [CU_CLEAN] a value tile loaded that passes the cleaning warps first
     uint64_t* r_full = dirty_full + CU_CLEAN;  // [CU_RING] unit published
     uint64_t* r_empty = r_full + CU_RING;
     auto ring = [&](int e) -> RingUnit& { return *reinterpret_cast<RingUnit*>(smem + C::UNIT_OFF + 64 * (e % CU_RING)); };
@@ -196,22 +211,22 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             uint32_t n = 1;
             if (b < empty) n = SRC == SRC_I8 ? C::HELPERS : 1;
             else if (b >= raw_empty && b < q_full) n = C::HELPERS;
-            else if (b >= q_full && b < q_empty) n = QF32 ? 4 : 1;
-            else if (b >= p_full && b < half_done) n = 4;
-            else if (b >= r_empty) n = 1 + 8 + C::HELPERS;  // product issuer, softmax warps, helpers
+            else if (b >= q_full && b < q_empty) n = QF32 ? C::SOFT / 2 : 1;
+            else if (b >= s_free && b < pv_done) n = C::SOFT / 2;
+            else if (b >= r_empty) n = (C::ALIAS ? 1 : 2) + C::SOFT + C::HELPERS;  // issuers, softmax warps, helpers
             mbar_init(b, n);
         }
         if (lane == 0) *s_abort = 0;
         fence_mbarrier_init();
     }
-    if (warp == 9) {
+    if (warp == C::SOFT + 1) {
         tc_alloc(s_tmem, 512);
         tc_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *s_tmem;  // columns: S/P of tile t at 128 t, O of tile t at 256 + D t
+    const uint32_t tmem = *s_tmem;
     pdl_wait();
     pdl_trigger();
 
@@ -224,31 +239,33 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
     };
     auto stop = [&]() { return __any_sync(0xffffffffu, *s_abort) != 0; };  // the same answer in a whole warp
 
-    if (warp < 8) {
+    if (warp < C::SOFT) {
         // ---------------------------------------------------------------- softmax, one thread per query row
         reg_alloc<C::REGS_SOFT>();
         const int t = warp >> 2;
         const int r = tid & 127;  // row of the tile
         const uint32_t lanes = uint32_t(warp & 3) << 21;  // this warp's quarter of the tensor-memory lanes
-        const uint32_t ts = tmem + lanes + 128 * t, to = tmem + lanes + 256 + D * t;
+        const uint32_t ts = tmem + lanes + 128 * (t % C::SBUFS), to = tmem + lanes + C::O_COL + D * t;
+        const uint32_t tp = C::ALIAS ? ts : tmem + lanes + 128 * C::SBUFS + 64 * t;
         const int tok = r / p.G, head = r % p.G;
         const int lp = SRC == SRC_I8 ? __ffs(p.page) - 1 : 0;
-        uint32_t ns = 0, no = 0;  // score tiles and units that this group has taken
+        uint32_t ns = 0, np = 0;  // scores taken, probabilities handed over
         uint32_t tiles = 0;       // key tiles of the CTA so far (int8 scale ring)
         constexpr int FOLD = QF32 ? CU_FOLD_F32 : CU_FOLD_F16;
         float4* fold = reinterpret_cast<float4*>(p.fold) + (size_t)(2 * blockIdx.x + t) * (D / 4) * 128 + r;
         for (int e = 0;; ++e) {
             wait(&r_full[e % CU_RING], e / CU_RING);
+            if (stop()) break;
             const RingUnit& R = ring(e);
             const ChunkUnit u = R.u;
             const int nt = R.nt[t], nall = max(R.nt[0], R.nt[1]), kt0 = R.t0;
-            if (u.state < 0 || stop()) break;
+            if (u.state < 0) break;
             auto leave = [&]() {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&r_empty[e % CU_RING]);
             };
             if (u.state == 2) {
-                if (t == 0) chunk_refuse<QT, D>(p, u, r, 128);
+                if (warp < 4) chunk_refuse<QT, D>(p, u, r, 128);
                 leave();
                 continue;
             }
@@ -268,7 +285,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             float f = p.q_scale;
             if constexpr (QF32) {
                 if (nt > 0) {
-                    // this row's query, split; the tile's previous scores are done (this group waited for them)
+                    // this row's query, split; the tile's previous scores are done (these warps waited for them)
                     const float4* q4 = reinterpret_cast<const float4*>(
                         static_cast<const float*>(p.q) + qrow * p.q_stride + (long long)h * D);
                     float amax = 0.f;
@@ -279,7 +296,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     }
                     // 2^-x amax in [1, 2) for a normal amax: exact, and the halves keep their 22 bits
                     int x = int(__float_as_uint(amax) >> 23) - 127;
-                    x = amax > 0.f && x < 128 ? max(x, -100) : 0;
+                    x = amax > 0.f && x < 128 ? min(max(x, -100), 126) : 0;
                     const float down = __uint_as_float(uint32_t(127 - x) << 23);
                     f *= __uint_as_float(uint32_t(127 + x) << 23);
                     uint8_t* qs = smem + C::Q_OFF + t * C::QTILE;
@@ -305,100 +322,119 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             float vexp = 0.f;       // int8: 2^-e, probabilities times the value scales times this; 0: not set
             float older = 1.f;      // what the folded sum has to be scaled by
             int folds = 0;
+            // every value product of this tile so far is done
+            auto settled = [&]() {
+                if (np > 0) wait(&pv_done[t], np - 1);
+                tc_fence_after();
+            };
             // O (complete up to here) and the folded sum times `scale`
             auto rescale = [&](float scale) {
                 older *= scale;
+                settled();
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    tc_ld32(to + c, o);
+                for (int c = 0; c < D; c += 16) {
+                    uint32_t o[16];
+                    tc_ld16(to + c, o);
                     tc_wait_ld();
-                    pin<32>(o);
+                    pin<16>(o);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * scale);
-                    tc_st32(to + c, o);
+                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * scale);
+                    tc_st16(to + c, o);
                 }
             };
+            bool lost = false;
             for (int j = 0; j < nt; ++j) {
-                if (__any_sync(0xffffffffu, !wait(&s_full[t], ns))) break;
-                tc_fence_after();
-                const int k0 = (kt0 + j) * CU_ROWS;
+                const int k0 = (kt0 + j) * CU_ROWS;  // first key
                 const bool masked = k0 + CU_ROWS > all_see;
-                const float* scales = s_scale + ((tiles + j) & 3) * 32;
-                if (j > 0 && j % FOLD == 0) {
-                    // the products of the tiles before are done, the next one starts O anew
-                    const bool plain = __all_sync(0xffffffffu, older == 1.f);
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t o[32];
-                        tc_ld32(to + c, o);
-                        tc_wait_ld();
-                        pin<32>(o);
-                        float4* at = fold + (c / 4) * 128;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i, at += 128) {
-                            float4 x = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                                   __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-                            if (folds == 0) {
-                                __stcg(at, x);
-                            } else if (plain) {
-                                asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(x.x), "f"(x.y),
-                                             "f"(x.z), "f"(x.w)
-                                             : "memory");
-                            } else {
-                                const float4 y = __ldcg(at);
-                                x.x = fmaf(y.x, older, x.x), x.y = fmaf(y.y, older, x.y);
-                                x.z = fmaf(y.z, older, x.z), x.w = fmaf(y.w, older, x.w);
-                                __stcg(at, x);
+                const float* scales = s_scale + (tiles + j) % C::SR * 32;
+                lost = __any_sync(0xffffffffu, !wait(&s_full[t], ns++)) != 0;
+                if (lost) break;
+                tc_fence_after();
+                // What O needs before the reference: waits for the value product before. The issuer reaches that
+                // one only after other scores, so with a shared score buffer this comes after s_free.
+                auto settle_outputs = [&]() {
+                    if (j > 0 && j % FOLD == 0) {
+                        // the next product starts O anew
+                        settled();
+                        const bool plain = __all_sync(0xffffffffu, older == 1.f);
+    #pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t o[16];
+                            tc_ld16(to + c, o);
+                            tc_wait_ld();
+                            pin<16>(o);
+                            float4* at = fold + (c / 4) * 128;
+    #pragma unroll
+                            for (int i = 0; i < 4; ++i, at += 128) {
+                                float4 x = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                       __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                                if (folds == 0) {
+                                    __stcg(at, x);
+                                } else if (plain) {
+                                    asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(x.x), "f"(x.y),
+                                                 "f"(x.z), "f"(x.w)
+                                                 : "memory");
+                                } else {
+                                    const float4 y = __ldcg(at);
+                                    x.x = fmaf(y.x, older, x.x), x.y = fmaf(y.y, older, x.y);
+                                    x.z = fmaf(y.z, older, x.z), x.w = fmaf(y.w, older, x.w);
+                                    __stcg(at, x);
+                                }
                             }
                         }
+                        ++folds;
+                        older = 1.f;
                     }
-                    ++folds;
-                    older = 1.f;
-                }
-                if constexpr (SRC == SRC_I8) {
-                    const float vm = s_vmax[(tiles + j) & 3];  // the tile's largest finite value scale
-                    if (vexp == 0.f || vm * vexp > 2.f) {      // (the same in every row)
-                        const int x = min(max(int(__float_as_uint(vm) >> 23) - 127, -100), 125);
-                        const float ve = __uint_as_float(uint32_t(126 - x) << 23);  // vm * ve in [0.5, 1)
-                        if (vexp != 0.f) rescale(ve / vexp);
-                        vexp = ve;
-                    }
-                }
-#pragma unroll 1
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t s[64];
-                    tc_ld32(ts + 64 * half, s);
-                    tc_ld32(ts + 64 * half + 32, s + 32);
-                    tc_wait_ld();
-                    pin<64>(s);
-                    const int kh = k0 + 64 * half;
                     if constexpr (SRC == SRC_I8) {
-#pragma unroll
-                        for (int c = 0; c < 64; c += 8) {
-                            const float ks = scales[(64 * half + c) >> lp];  // (pages of 128 tokens or more: one)
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) s[c + i] = __float_as_uint(__uint_as_float(s[c + i]) * ks);
+                        const float vm = s_vmax[(tiles + j) % C::SR];  // the tile's largest finite value scale
+                        if (vexp == 0.f || vm * vexp > 2.f) {          // (the same in every row)
+                            const int x = min(max(int(__float_as_uint(vm) >> 23) - 127, -100), 125);
+                            const float ve = __uint_as_float(uint32_t(126 - x) << 23);  // vm * ve in [0.5, 1)
+                            if (vexp != 0.f) rescale(ve / vexp);
+                            vexp = ve;
                         }
                     }
-                    if (masked) {
-                        const int lim = limit - kh;
+                };
+                // the scores move to registers at once; with a buffer of their own it is free for the next ones
+                uint32_t s[CU_ROWS];
 #pragma unroll
-                        for (int c = 0; c < 64; ++c)
-                            if (c >= lim) s[c] = 0xff800000u;  // -inf
+                for (int c0 = 0; c0 < CU_ROWS; c0 += 32) tc_ld32(ts + c0, s + c0);
+                tc_wait_ld();
+                pin<CU_ROWS>(s);
+                if constexpr (!C::ALIAS) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_free[t % C::SBUFS]);
+                }
+                settle_outputs();
+                if constexpr (SRC == SRC_I8) {
+#pragma unroll
+                    for (int c = 0; c < CU_ROWS; c += 8) {
+                        const float ks = scales[c >> lp];  // (pages of 128 tokens or more: one)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) s[c + i] = __float_as_uint(__uint_as_float(s[c + i]) * ks);
                     }
-                    uint32_t pr[QF32 ? 64 : 32];
-                    float sum, mt;
-                    auto probabilities = [&](float base) {
-                        const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
-                        uint64_t l0 = 0, l1 = 0;
-                        float m0 = -INFINITY, m1 = -INFINITY;
+                }
+                if (masked) {
+                    const int lim = limit - k0;
 #pragma unroll
-                        for (int i = 0; i < 64; i += 2) {
-                            const float s0 = __uint_as_float(s[i]), s1 = __uint_as_float(s[i + 1]);
-                            if (i & 2) m1 = max3_nan(m1, s0, s1);
-                            else m0 = max3_nan(m0, s0, s1);
-                            const uint64_t x = fma2(pack2(s0, s1), f2, b2);
+                    for (int c = 0; c < CU_ROWS; ++c)
+                        if (c >= lim) s[c] = 0xff800000u;  // -inf
+                }
+                settled();  // the product that reads the probabilities before these
+                // The probabilities to tensor memory (QF32: hi, then lo halves of 32 keys, 16 columns each);
+                // their sum.
+                auto probabilities = [&]() {
+                    const float base = ref == -INFINITY ? 0.f : -ref;
+                    const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
+                    uint64_t l0 = 0, l1 = 0;
+#pragma unroll
+                    for (int c0 = 0; c0 < CU_ROWS; c0 += 32) {
+                        uint32_t pr[QF32 ? 32 : 16];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const uint64_t x =
+                                fma2(pack2(__uint_as_float(s[c0 + i]), __uint_as_float(s[c0 + i + 1])), f2, b2);
                             float a, b;
                             if (!QF32 && (i / 2) % CU_POLY_OF < CU_POLY) {
                                 exp2_poly2(x, a, b);
@@ -410,73 +446,57 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                             if (i & 2) l1 = add2(l1, pack2(a, b));
                             else l0 = add2(l0, pack2(a, b));
                             if constexpr (SRC == SRC_I8) {
-                                const float vs = scales[16 + ((64 * half + i) >> lp)] * vexp;
+                                const float vs = scales[16 + ((c0 + i) >> lp)] * vexp;
                                 a *= vs;
                                 b *= vs;
                                 if (masked) {  // the scale of a page that this row does not see may be anything
-                                    if (kh + i >= limit) a = 0.f;
-                                    if (kh + i + 1 >= limit) b = 0.f;
+                                    if (k0 + c0 + i >= limit) a = 0.f;
+                                    if (k0 + c0 + i + 1 >= limit) b = 0.f;
                                 }
                             }
-                            if constexpr (QF32) split_hi_lo(a, b, pr[32 * (i / 32) + i % 32 / 2], pr[32 * (i / 32) + 16 + i % 32 / 2]);
+                            if constexpr (QF32) split_hi_lo(a, b, pr[i / 2], pr[16 + i / 2]);
                             else pr[i / 2] = h2_as_u32(__floats2half2_rn(a, b));
                         }
-                        float a, b;
-                        unpack2(add2(l0, l1), a, b);
-                        sum = a + b;
-                        mt = fmaxf_nan(m0, m1);
-                    };
-                    bool move = j == 0 && half == 0;
-                    if (!move) {
-                        probabilities(ref == -INFINITY ? 0.f : -ref);
-                        move = mt * f - CU_SHIFT > ref + CU_TAU;
-                    } else {
-                        float m0 = -INFINITY, m1 = -INFINITY;
+                        if constexpr (QF32) tc_st32(tp + c0, pr);
+                        else tc_st16(tp + c0 / 2, pr);
+                    }
+                    float a, b;
+                    unpack2(add2(l0, l1), a, b);
+                    return a + b;
+                };
+                // With the reference so far first. No probability is above their sum, so a sum in bounds needs
+                // no maximum. Otherwise (NaN included) the reference rises to the highest score, O and l
+                // follow, and the probabilities are computed again.
+                float sum = 0.f;
+                if (j > 0) sum = probabilities();
+                if (j == 0 || __any_sync(0xffffffffu, !(sum <= CU_MOST))) {
+                    float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < 64; i += 4) {
-                            m0 = max3_nan(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                            m1 = max3_nan(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
-                        }
-                        mt = fmaxf_nan(m0, m1);
+                    for (int i = 0; i < CU_ROWS; i += 4) {
+                        m0 = max3_nan(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                        m1 = max3_nan(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
                     }
-                    if (__any_sync(0xffffffffu, move)) {
-                        // a new reference where a score passed the old one: O, l and these probabilities follow
-                        float scale = 1.f;
-                        const float top = mt * f - CU_SHIFT;
-                        if (top > ref) {
-                            scale = ref == -INFINITY ? 0.f : ex2(ref - top);
-                            ref = top;
-                            l *= scale;
-                        }
-                        if (j > 0 || half) {
-                            if (half) wait(&half_done[t], ns);
-                            tc_fence_after();
-                            rescale(scale);
-                        }
-                        probabilities(ref == -INFINITY ? 0.f : -ref);
+                    const float top = fmaxf_nan(m0, m1) * f - CU_SHIFT;
+                    float scale = 1.f;
+                    if (top > ref) {
+                        scale = ref == -INFINITY ? 0.f : ex2(ref - top);
+                        ref = top;
+                        l *= scale;
                     }
-                    // a NaN or +inf score makes the whole row NaN
-                    l += mt < INFINITY ? sum : __int_as_float(0x7fc00000);
-                    if constexpr (QF32) {  // hi, lo of 32 keys: 16 columns each
-                        tc_st32(ts + 64 * half, pr);
-                        tc_st32(ts + 64 * half + 32, pr + 32);
-                    } else {
-                        tc_st32(ts + 32 * half, pr);
-                    }
-                    tc_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[2 * t + half]);
+                    if (j > 0) rescale(scale);
+                    sum = probabilities();
+                    if (!(top < INFINITY)) sum = __int_as_float(0x7fc00000);  // a NaN or +inf score: the row is NaN
                 }
-                ++ns;
+                l += sum;
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[t]);
+                ++np;
             }
+            if (lost) break;
             tiles += nall;
-            if (nt > 0) {
-                wait(&o_full[t], no);
-                ++no;
-                tc_fence_after();
-            }
-            if (stop()) break;
+            settled();
             const volatile RingUnit& V = R;
             const bool bad = V.bad != 0, odd = V.odd != 0;
             if (bad && r == 0) raise_error(p.error_flag, KVB_DEVERR_BLOCK);
@@ -539,7 +559,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
         }
     } else {
         reg_dealloc<C::REGS_REST>();
-        if (warp == 8) {
+        if (warp == C::SOFT) {
             // ------------------------------------------------------------ producer and scheduler
             const uint64_t policy = l2_evict_first_policy();
             uint32_t item = 0, tiles = 0, units = 0;
@@ -585,115 +605,119 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 const int bt = SRC == SRC_PACKED ? CU_ROWS : min(p.page, CU_ROWS);  // keys of a box
                 const int nbox = CU_ROWS / bt;
                 const int* table = p.block_table + (SRC == SRC_PACKED ? 0 : (size_t)u.b * p.max_blocks);
-                // the block id (int8: and scales) of this lane's box of a tile, one tile ahead
-                int id = -1, nid = -1;
+                // Items: K of tile 0, then K of the next tile and V of this one in turn, V of the last tile:
+                // scores run a tile ahead of the values. The block id of this lane's box of a tile is read a
+                // tile ahead.
                 auto fetch = [&](int j) {
                     const int k = (range.x + j) * CU_ROWS + lane * bt;
                     return SRC != SRC_PACKED && j < nj && lane < nbox && k < u.keys ? __ldg(table + k / p.page) : -1;
                 };
-                nid = fetch(0);
-                for (int j = 0; j < nj && !stop(); ++j) {
-                    id = nid;
-                    nid = fetch(j + 1);
+                int id_v = -1, id_k = fetch(0), id_n = fetch(1);  // of the value tile, the key tile, the next one
+                for (int i = 0; i < 2 * nj && !stop(); ++i) {
+                    const bool is_v = i == 2 * nj - 1 || (i > 0 && i % 2 == 0);
+                    const int j = is_v ? (i == 2 * nj - 1 ? nj - 1 : i / 2 - 1) : (i + 1) / 2;
+                    if (!is_v && i > 0) {
+                        id_v = id_k;
+                        id_k = id_n;
+                        id_n = fetch(j + 1);
+                    }
+                    if (i == 2 * nj - 1) id_v = id_k;
+                    const int id = is_v ? id_v : id_k;
                     const int k = (range.x + j) * CU_ROWS + lane * bt;
                     const bool wanted = SRC != SRC_PACKED && lane < nbox && k < u.keys;
                     const bool ok = wanted && id >= 0 && id < p.num_blocks;
-                    if (__any_sync(0xffffffffu, wanted && !ok) && lane == 0)
+                    if (!is_v && __any_sync(0xffffffffu, wanted && !ok) && lane == 0)
                         reinterpret_cast<volatile RingUnit&>(ring(e)).bad = 1;
                     const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, ok));
                     if constexpr (SRC == SRC_I8) {
+                        const uint32_t st = item % C::NR;
                         float ks = 0.f, vs = 0.f;
-                        if (ok) {
+                        if (ok && !is_v) {
                             ks = __ldg(p.k_scale + (long long)id * p.Hkv + u.kvh);
                             vs = __ldg(p.v_scale + (long long)id * p.Hkv + u.kvh);
                         }
-                        // the ring's slot: its readers are done, since the item six before this one is
-                        if (item >= C::NR) wait(&raw_empty[item % C::NR], item / C::NR - 1);
-                        const float vm = warp_max(vs <= 3.402823466e38f ? vs : 0.f);
-                        if (lane < 16) {
-                            s_scale[(tiles & 3) * 32 + lane] = ks;
-                            s_scale[(tiles & 3) * 32 + 16 + lane] = vs;
+                        if (item >= C::NR) wait(&raw_empty[st], item / C::NR - 1);
+                        if (!is_v) {
+                            // (the slot's readers are done: of the six items in flight at most, three are keys)
+                            const float vm = warp_max(vs <= 3.402823466e38f ? vs : 0.f);
+                            if (lane < 16) {
+                                s_scale[tiles % C::SR * 32 + lane] = ks;
+                                s_scale[tiles % C::SR * 32 + 16 + lane] = vs;
+                            }
+                            if (lane == 0) s_vmax[tiles % C::SR] = vm;
+                            ++tiles;
                         }
-                        if (lane == 0) s_vmax[tiles & 3] = vm;
-                    }
-#pragma unroll
-                    for (int which = 0; which < 2; ++which) {  // K, then V
-                        if constexpr (SRC == SRC_I8) {
-                            const uint32_t st = item % C::NR;
-                            if (item >= C::NR) wait(&raw_empty[st], item / C::NR - 1);
-                            __syncwarp();
-                            const uint32_t bytes = uint32_t(bt) * D;
+                        __syncwarp();
+                        const uint32_t bytes = uint32_t(bt) * D;
+                        if (lane == 0) {
+                            if (boxes && !*s_abort) mbar_arrive_expect_tx(&raw_full[st], boxes * bytes);
+                            else mbar_arrive(&raw_full[st]);
+                        }
+                        __syncwarp();
+                        if (ok && !*s_abort) {
+                            const int8_t* src = static_cast<const int8_t*>(is_v ? p.v : p.k) +
+                                                (((long long)id * p.Hkv + u.kvh) * p.page + k % p.page) * D;
+                            bulk_load(smem + C::RAW_OFF + st * C::RAW + lane * bytes, src, bytes, &raw_full[st]);
+                        }
+                    } else {
+                        const uint32_t st = item % NS;
+                        if (item >= NS) wait(&empty[st], item / NS - 1);
+                        __syncwarp();
+                        uint8_t* dst = smem + C::KV_OFF + st * C::ITEM;
+                        const CUtensorMap* map = is_v ? &tmv : &tmk;
+                        uint64_t* done = &full[st];
+                        if (is_v && j >= dirty) done = &dirty_full[dirty_n++ % CU_CLEAN];
+                        if constexpr (SRC == SRC_PACKED) {
                             if (lane == 0) {
-                                if (boxes && !*s_abort) mbar_arrive_expect_tx(&raw_full[st], boxes * bytes);
-                                else mbar_arrive(&raw_full[st]);
+                                if (*s_abort) {
+                                    mbar_arrive(done);
+                                } else {
+                                    mbar_arrive_expect_tx(done, C::ITEM);
+#pragma unroll
+                                    for (int s = 0; s < NSUB; ++s)
+                                        tma_load_3d(dst + s * CU_SUB, map, done, 64 * s, u.kvh,
+                                                    u.kv0 + (range.x + j) * CU_ROWS);
+                                }
+                            }
+                        } else {
+                            if (lane == 0) {
+                                if (boxes && !*s_abort) mbar_arrive_expect_tx(done, boxes * bt * 128 * NSUB);
+                                else mbar_arrive(done);
                             }
                             __syncwarp();
                             if (ok && !*s_abort) {
-                                const int8_t* src = static_cast<const int8_t*>(which ? p.v : p.k) +
-                                                    (((long long)id * p.Hkv + u.kvh) * p.page + k % p.page) * D;
-                                bulk_load(smem + C::RAW_OFF + st * C::RAW + lane * bytes, src, bytes, &raw_full[st]);
+                                const int y = (id * p.Hkv + u.kvh) * p.page + k % p.page;
+#pragma unroll
+                                for (int s = 0; s < NSUB; ++s)
+                                    tma_load_2d(dst + s * CU_SUB + lane * bt * 128, map, done, 64 * s, y, policy);
                             }
-                        } else {
-                            const uint32_t st = item % NS;
-                            if (item >= NS) wait(&empty[st], item / NS - 1);
-                            __syncwarp();
-                            uint8_t* dst = smem + C::KV_OFF + st * C::ITEM;
-                            const CUtensorMap* map = which ? &tmv : &tmk;
-                            uint64_t* done = &full[st];
-                            if (which && j >= dirty) done = &dirty_full[dirty_n++ % CU_CLEAN];
-                            if constexpr (SRC == SRC_PACKED) {
-                                if (lane == 0) {
-                                    if (*s_abort) {
-                                        mbar_arrive(done);
-                                    } else {
-                                        mbar_arrive_expect_tx(done, C::ITEM);
-#pragma unroll
-                                        for (int i = 0; i < NSUB; ++i)
-                                            tma_load_3d(dst + i * CU_SUB, map, done, 64 * i, u.kvh,
-                                                        u.kv0 + (range.x + j) * CU_ROWS);
-                                    }
-                                }
-                            } else {
-                                if (lane == 0) {
-                                    if (boxes && !*s_abort) mbar_arrive_expect_tx(done, boxes * bt * 128 * NSUB);
-                                    else mbar_arrive(done);
-                                }
-                                __syncwarp();
-                                if (ok && !*s_abort) {
-                                    const int y = (id * p.Hkv + u.kvh) * p.page + k % p.page;
-#pragma unroll
-                                    for (int i = 0; i < NSUB; ++i)
-                                        tma_load_2d(dst + i * CU_SUB + lane * bt * 128, map, done, 64 * i, y, policy);
-                                }
-                            }
-                        }
-                        ++item;
-                        if (!QF32 && j == 0 && which == 0) {
-                            // the queries, once the unit before has used its own
-                            if (qn > 0) wait(q_empty, qn - 1);
-                            ++qn;
-                            if (lane == 0 && !*s_abort) {
-                                const uint32_t bytes = uint32_t(p.tile_tokens * p.G) * 128 * NSUB;
-#pragma unroll
-                                for (int t = 0; t < 2; ++t) {
-                                    if ((t ? nt1 : nt0) == 0) continue;
-                                    mbar_arrive_expect_tx(&q_full[t], bytes);
-#pragma unroll
-                                    for (int i = 0; i < NSUB; ++i)
-                                        tma_load_3d(smem + C::Q_OFF + t * C::QTILE + i * CU_SUB, &tmq, &q_full[t], 64 * i,
-                                                    u.kvh * p.G, u.row0 + t * p.tile_tokens);
-                                }
-                            }
-                            __syncwarp();
                         }
                     }
-                    ++tiles;
+                    ++item;
+                    if (!QF32 && i == 0) {
+                        // the queries, once the unit before has used its own
+                        if (qn > 0) wait(q_empty, qn - 1);
+                        ++qn;
+                        if (lane == 0 && !*s_abort) {
+                            const uint32_t bytes = uint32_t(p.tile_tokens * p.G) * 128 * NSUB;
+#pragma unroll
+                            for (int t = 0; t < 2; ++t) {
+                                if ((t ? nt1 : nt0) == 0) continue;
+                                mbar_arrive_expect_tx(&q_full[t], bytes);
+#pragma unroll
+                                for (int s = 0; s < NSUB; ++s)
+                                    tma_load_3d(smem + C::Q_OFF + t * C::QTILE + s * CU_SUB, &tmq, &q_full[t], 64 * s,
+                                                u.kvh * p.G, u.row0 + t * p.tile_tokens);
+                            }
+                        }
+                        __syncwarp();
+                    }
                 }
             }
             ChunkUnit end{};
             end.state = -1;
             publish(end, make_int2(0, 0), 0, 0);
-        } else if (warp == 9) {
+        } else if (warp == C::SOFT + 1 || (warp == C::SOFT + 2 && !C::ALIAS)) {
             // ------------------------------------------------------------ products
             if (tc_elect()) {
                 constexpr uint32_t id_s = instr_desc(1, 0, 0, 0, 0, 128, 128);
@@ -703,32 +727,40 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 const uint64_t kd = smem_desc(sbase + uint32_t(C::KV_OFF), 16, 1024);
                 const uint64_t vd = smem_desc(sbase + uint32_t(C::KV_OFF), CU_SUB, 1024);
                 const uint64_t qd = smem_desc(sbase + uint32_t(C::Q_OFF), 16, 1024);
-                uint32_t item = 0, nq0 = 0, nq1 = 0, np0 = 0, np1 = 0;
+                uint32_t item = 0;                // first item of the unit
+                uint32_t nq0 = 0, nq1 = 0, np0 = 0, np1 = 0, nb0 = 0, nb1 = 0;  // uses of each barrier
                 auto scores = [&](int t, uint32_t it) {
+                    if constexpr (!C::ALIAS) {  // the buffer's scores before these were read
+                        uint32_t& nb = t % C::SBUFS ? nb1 : nb0;
+                        if (nb > 0) wait(&s_free[t % C::SBUFS], nb - 1);
+                        ++nb;
+                    }
+                    tc_fence_after();
                     const uint64_t k = kd + (it % NS) * (C::ITEM / 16), q = qd + t * (C::QTILE / 16);
 #pragma unroll
                     for (int part = 0; part < (QF32 ? 2 : 1); ++part)
 #pragma unroll
                         for (int i = 0; i < D / 16; ++i) {
                             const uint32_t off = ((i / 4) * CU_SUB + (i % 4) * 32) / 16;
-                            tc_mma<1>(tmem + 128 * t, q + (part * NSUB * CU_SUB / 16 + off), k + off, id_s, part > 0 || i > 0);
+                            tc_mma<1>(tmem + 128 * (t % C::SBUFS), q + (part * NSUB * CU_SUB / 16 + off), k + off, id_s, part > 0 || i > 0);
                         }
                     tc_commit(&s_full[t]);
                 };
-                auto values = [&](int t, uint32_t it, int half, bool keep) {
-                    const uint64_t v = vd + (it % NS) * (C::ITEM / 16) + half * (64 * 128 / 16);
-                    const uint32_t ts = tmem + 128 * t + (QF32 ? 64 : 32) * half, to = tmem + 256 + D * t;
+                auto values = [&](int t, uint32_t it, bool keep) {
+                    const uint64_t v = vd + (it % NS) * (C::ITEM / 16);
+                    const uint32_t tp = tmem + (C::ALIAS ? 128 * t : 128 * C::SBUFS + 64 * t), to = tmem + C::O_COL + D * t;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < CU_ROWS / 16; ++i) {
                         const uint64_t b = v + i * (2048 / 16);
                         if constexpr (QF32) {
-                            const uint32_t a = ts + 32 * (i / 2) + 8 * (i % 2);
+                            const uint32_t a = tp + 32 * (i / 2) + 8 * (i % 2);
                             tc_mma_ts(to, a, b, id_o, keep || i > 0);
                             tc_mma_ts(to, a + 16, b, id_o, 1);
                         } else {
-                            tc_mma_ts(to, ts + 8 * i, b, id_o, keep || i > 0);
+                            tc_mma_ts(to, tp + 8 * i, b, id_o, keep || i > 0);
                         }
                     }
+                    tc_commit(&pv_done[t]);
                 };
                 auto ready = [&](uint32_t it) { return wait(&full[it % NS], it / NS); };
                 for (int e = 0; !*s_abort; ++e) {
@@ -739,49 +771,59 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     if (state < 0) break;
                     const int nj = max(nt0, nt1);
                     if (nj == 0) continue;
-                    // K of key tile j is item `item` + 2 j, its V the next one
-                    ready(item);
-                    if (nt0 > 0) {
-                        wait(&q_full[0], nq0++);
+                    auto key_item = [&](int j) { return item + (j == 0 ? 0 : 2 * j - 1); };
+                    auto value_item = [&](int j) { return item + min(2 * j + 2, 2 * nj - 1); };
+                    auto score_step = [&](int t, int j) {
+                        if (j >= (t ? nt1 : nt0)) return;
+                        if (j == 0) wait(&q_full[t], t ? nq1++ : nq0++);
+                        scores(t, key_item(j));
+                    };
+                    auto value_step = [&](int t, int j) {
+                        if (j >= (t ? nt1 : nt0)) return;
+                        if (!wait(&p_full[t], t ? np1++ : np0++)) return;
                         tc_fence_after();
-                        scores(0, item);
-                    }
-                    if (nt1 > 0) {
-                        wait(&q_full[1], nq1++);
-                        tc_fence_after();
-                        scores(1, item);
-                    }
-                    tc_commit(&empty[item % NS]);
-                    if (nj == 1) tc_commit(q_empty);
-                    for (int j = 0; j < nj && !*s_abort; ++j) {
-                        const uint32_t iv = item + 1, ik = item + 2;
-                        bool have_k = false;
-                        ready(iv);
-#pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            const int nt = t ? nt1 : nt0;
-                            if (j >= nt) continue;
-                            uint32_t& np = t ? np1 : np0;
-                            if (!wait(&p_full[2 * t], np)) break;
-                            tc_fence_after();
-                            values(t, iv, 0, j % FOLD != 0);
-                            tc_commit(&half_done[t]);
-                            if (j + 1 < nt && !have_k) have_k = ready(ik);  // while the second half is computed
-                            if (!wait(&p_full[2 * t + 1], np)) break;
-                            tc_fence_after();
-                            values(t, iv, 1, true);
-                            ++np;
-                            if (j + 1 < nt) {
-                                scores(t, ik);
-                            } else {
-                                tc_commit(&o_full[t]);
-                            }
+                        values(t, value_item(j), j % FOLD != 0);
+                    };
+                    // the stages of a key (value) tile, once both query tiles' products with it are issued
+                    auto keys_done = [&](int j) {
+                        tc_commit(&empty[key_item(j) % NS]);
+                        if (j + 1 == nj) tc_commit(q_empty);
+                    };
+                    if constexpr (C::ALIAS) {
+                        // a tile's next scores overwrite its probabilities, so they follow its value product
+                        ready(key_item(0));
+                        score_step(0, 0);
+                        score_step(1, 0);
+                        keys_done(0);
+                        for (int j = 0; j < nj && !*s_abort; ++j) {
+                            const bool more = j + 1 < nj;
+                            if (more) ready(key_item(j + 1));
+                            ready(value_item(j));
+                            value_step(0, j);
+                            score_step(0, j + 1);
+                            value_step(1, j);
+                            score_step(1, j + 1);
+                            tc_commit(&empty[value_item(j) % NS]);
+                            if (more) keys_done(j + 1);
                         }
-                        tc_commit(&empty[iv % NS]);
-                        if (j + 1 < nj) tc_commit(&empty[ik % NS]);
-                        if (j + 2 == nj) tc_commit(q_empty);
-                        item += 2;
+                    } else if (warp == C::SOFT + 1) {
+                        // scores go out as soon as their buffer was read
+                        for (int j = 0; j < nj && !*s_abort; ++j) {
+                            ready(key_item(j));
+                            score_step(0, j);
+                            score_step(1, j);
+                            keys_done(j);
+                        }
+                    } else {
+                        // value products as soon as the probabilities are there
+                        for (int j = 0; j < nj && !*s_abort; ++j) {
+                            ready(value_item(j));
+                            value_step(0, j);
+                            value_step(1, j);
+                            tc_commit(&empty[value_item(j) % NS]);
+                        }
                     }
+                    item += 2 * nj;
                 }
             }
         } else if (warp >= C::HELPER0) {
@@ -831,7 +873,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     // (the two warps take them in turn)
                     for (int j = max(0, dirty); j < nj && !stop(); ++j, ++cleaned) {
                         if (int(cleaned % C::HELPERS) != ht >> 5) continue;
-                        const uint32_t it = item + 2 * j + 1;
+                        const uint32_t it = item + min(2 * j + 2, 2 * nj - 1);
                         wait(&dirty_full[cleaned % CU_CLEAN], cleaned / CU_CLEAN);
                         uint8_t* v = smem + C::KV_OFF + (it % NS) * C::ITEM;
                         const int live_rows = keys - (kt0 + j) * CU_ROWS;  // rows from here on no token sees
@@ -876,7 +918,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 9) tc_dealloc(tmem, 512);
+    if (warp == C::SOFT + 1) tc_dealloc(tmem, 512);
     if (tid == 0 && *s_abort) raise_error(p.error_flag, KVB_DEVERR_TIMEOUT);
 }
 
