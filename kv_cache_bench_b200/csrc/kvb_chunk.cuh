@@ -25,8 +25,10 @@ struct ChunkParams {
     unsigned* error_flag;
     float* part_o;              // splits > 1: [splits][T][H][D], each split's normalized output
     float2* part_ml;            // [splits][T][H]: (max in log2 units, sum); a NaN sum: refused
+                                // tcgen05 kernel: [2 ctas][2 tiles][128 rows] ([D]): the CTAs' partial units
     float* fold;                // tcgen05 kernel, long keys: each CTA's running sums [2 tiles][D / 4][128][4]
-    unsigned* next_unit;        // dynamic hand-out (zeroed before the launch), or null
+    struct ChunkPiece* pieces;  // tcgen05 kernel: [ctas]
+    int ctas;                   // tcgen05 kernel: CTAs that share the work
     long long num_blocks;
     int B, H, Hkv, G, T;
     int page, max_blocks, max_new, max_len;
@@ -42,12 +44,21 @@ struct ChunkParams {
 #define KVB_CHUNK_FOLD_F32 8
 #define KVB_CHUNK_FOLD_F16 64
 
+// What a CTA of the tcgen05 kernel leaves for the merge: the unit whose first keys it took and whose others
+// the next CTAs did, and whether it took later keys of a unit that an earlier CTA began.
+struct ChunkPiece {
+    int kvh, row0, n;  // the unit: KV head, first token, tokens
+    int last;          // last CTA with keys of it; -1: this CTA began no such unit
+    int head;          // it has such later keys
+};
+
 // Whether the tcgen05 kernel takes the call.
 bool kvb_chunk_umma_supported(int q_type, int kv_type, bool paged, int D, int page, int G);
 cudaError_t kvb_launch_chunk_umma(const ChunkParams& p, int q_type, int kv_type, int D, const void* tmap_q,
-                                  const void* tmap_k, const void* tmap_v, int num_sms, cudaStream_t stream);
+                                  const void* tmap_k, const void* tmap_v, cudaStream_t stream);
 cudaError_t kvb_launch_chunk_simt(const ChunkParams& p, int q_type, int kv_type, int D, cudaStream_t stream);
 cudaError_t kvb_launch_chunk_merge(const ChunkParams& p, int q_type, int D, int num_sms, cudaStream_t stream);
+cudaError_t kvb_launch_chunk_join(const ChunkParams& p, int q_type, int D, cudaStream_t stream);
 // New tokens and units of the two kernels' query tiles.
 constexpr int KVB_SIMT_ROWS = 64;
 
@@ -65,6 +76,30 @@ struct ChunkUnit {
     int state;     // 0: work, 1: no unit here, 2: refused: rows [row0, row0 + n) become NaN
 };
 
+// A sequence's place in a call, checked.
+struct ChunkSeq {
+    int c0, n, ctx;  // first packed row, new tokens, keys before them
+    bool bad;
+};
+
+__device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams& p, int b) {
+    const int c0 = __ldg(p.cu + b), c1 = __ldg(p.cu + b + 1);
+    const long long n = (long long)c1 - c0;
+    const long long total = p.block_table ? __ldg(p.total_lens + b) : n;
+    ChunkSeq s;
+    s.bad = c0 < 0 || n < 0 || c1 > p.T || n > p.max_new || (n > 0 && total < n) || total > p.max_len ||
+            (p.block_table && total > (long long)p.max_blocks * p.page);
+    s.c0 = c0;
+    s.n = int(n);
+    s.ctx = int(total - n);
+    if (s.bad) {
+        s.c0 = min(max(c0, 0), p.T);
+        s.n = max(0, min(max(c1, 0), p.T) - s.c0);
+        s.ctx = 0;
+    }
+    return s;
+}
+
 // Units are numbered with the last tokens of the sequences first: they see the most keys, so the
 // longest units start first and the short ones fill the end.
 __device__ __forceinline__ ChunkUnit chunk_unit(const ChunkParams& p, long long idx) {
@@ -75,28 +110,22 @@ __device__ __forceinline__ ChunkUnit chunk_unit(const ChunkParams& p, long long 
     r /= p.splits;
     u.b = int(r % p.B);
     const int blk = p.blocks_of_new - 1 - int(r / p.B);
-    const int c0 = __ldg(p.cu + u.b), c1 = __ldg(p.cu + u.b + 1);
-    const long long n = (long long)c1 - c0;
-    const long long total = p.block_table ? __ldg(p.total_lens + u.b) : n;
-    const bool bad = c0 < 0 || n < 0 || c1 > p.T || n > p.max_new || (n > 0 && total < n) || total > p.max_len ||
-                     (p.block_table && total > (long long)p.max_blocks * p.page);
-    u.row0 = u.kv0 = c0;
+    const ChunkSeq s = chunk_seq(p, u.b);
+    u.row0 = u.kv0 = s.c0;
     u.state = 1;
     u.n = u.pos0 = u.keys = 0;
-    if (bad) {
+    if (s.bad) {
         if (blk != 0) return u;
-        const int a = min(max(c0, 0), p.T), z = min(max(c1, 0), p.T);
         u.state = 2;
-        u.row0 = a;
-        u.n = max(0, z - a);
+        u.n = s.n;
         return u;
     }
     const int t0 = blk * p.unit_tokens;
-    if (t0 >= n) return u;
+    if (t0 >= s.n) return u;
     u.state = 0;
-    u.row0 = c0 + t0;
-    u.n = min(p.unit_tokens, int(n) - t0);
-    u.pos0 = int(total - n) + t0;
+    u.row0 = s.c0 + t0;
+    u.n = min(p.unit_tokens, s.n - t0);
+    u.pos0 = s.ctx + t0;
     u.keys = u.pos0 + u.n;
     return u;
 }

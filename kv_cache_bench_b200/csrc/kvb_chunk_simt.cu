@@ -315,6 +315,74 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const __grid_constant_
     }
 }
 
+// Joins the pieces of the units that the tcgen05 kernel's CTAs cut: CTA (c, y) takes the unit that part c
+// began, rows 32 y .. 32 y + 31 of its two query tiles, a warp a row: the piece of part c and those of the
+// parts behind it up to the unit's last.
+template <typename QT, int D>
+__global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__ ChunkParams p) {
+    constexpr int E = D / 32;
+    using V = typename std::conditional<E == 4, float4, float2>::type;
+    const int lane = threadIdx.x & 31, c = blockIdx.x;
+    pdl_wait();
+    pdl_trigger();
+    const ChunkPiece u = p.pieces[c];
+    if (u.last < 0) return;
+#pragma unroll 1
+    for (int i = threadIdx.x >> 5; i < 32; i += 8) {
+        const int rr = blockIdx.y * 32 + i, t = rr / 128, r = rr % 128;
+        const int tok = t * p.tile_tokens + r / p.G;
+        if (r >= p.tile_tokens * p.G || tok >= u.n) continue;
+        float M = -INFINITY, S = 0.f, A[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) A[e] = 0.f;
+        constexpr int U = 4;
+        for (int k0 = c; k0 <= u.last; k0 += U) {
+            float2 ml[U];
+            V x[U];
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const int k = k0 + j;
+                ml[j] = make_float2(-INFINITY, 0.f);
+                if (k <= u.last && (k == c || p.pieces[k].head)) {
+                    const long long at = ((long long)(k == c ? 2 * k + 1 : 2 * k) * 2 + t) * 128 + r;
+                    ml[j] = __ldcg(p.part_ml + at);
+                    x[j] = __ldcg(reinterpret_cast<const V*>(p.part_o + at * D) + lane);
+                }
+            }
+            float Mb = M;
+#pragma unroll
+            for (int j = 0; j < U; ++j) Mb = fmaxf(Mb, ml[j].x);
+            const float sc = M == Mb ? 1.f : exp2f(M - Mb);
+            S *= sc;
+#pragma unroll
+            for (int e = 0; e < E; ++e) A[e] *= sc;
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                if (ml[j].y == 0.f) continue;  // a piece without keys that this row sees
+                const float w = ml[j].y * exp2f(ml[j].x - Mb);
+                S += w;
+                const float* f = reinterpret_cast<const float*>(&x[j]);
+#pragma unroll
+                for (int e = 0; e < E; ++e) A[e] = fmaf(w, f[e], A[e]);
+            }
+            M = Mb;
+        }
+        const float inv = 1.f / S;
+        QT* out = static_cast<QT*>(p.out) + ((size_t)(u.row0 + tok) * p.H + u.kvh * p.G + r % p.G) * D + lane * E;
+        if constexpr (sizeof(QT) == 4) {
+            V y;
+            float* f = reinterpret_cast<float*>(&y);
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[e] = A[e] * inv;
+            *reinterpret_cast<V*>(out) = y;
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e += 2)
+                *reinterpret_cast<__half2*>(out + e) = __floats2half2_rn(A[e] * inv, A[e + 1] * inv);
+        }
+    }
+}
+
 template <typename QT, typename KT, int D>
 cudaError_t launch(const ChunkParams& p, cudaStream_t stream) {
     using C = SimtCfg<D>;
@@ -354,4 +422,21 @@ cudaError_t kvb_launch_chunk_merge(const ChunkParams& p, int q_type, int D, int 
                         : kvb_launch_pdl(chunk_merge_kernel<float, 64>, grid, 256, 0, stream, p);
     return D == 128 ? kvb_launch_pdl(chunk_merge_kernel<__half, 128>, grid, 256, 0, stream, p)
                     : kvb_launch_pdl(chunk_merge_kernel<__half, 64>, grid, 256, 0, stream, p);
+}
+
+cudaError_t kvb_launch_chunk_join(const ChunkParams& p, int q_type, int D, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.ctas, 8);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (q_type == KVB_F32)
+        return D == 128 ? cudaLaunchKernelEx(&cfg, chunk_join_kernel<float, 128>, p)
+                        : cudaLaunchKernelEx(&cfg, chunk_join_kernel<float, 64>, p);
+    return D == 128 ? cudaLaunchKernelEx(&cfg, chunk_join_kernel<__half, 128>, p)
+                    : cudaLaunchKernelEx(&cfg, chunk_join_kernel<__half, 64>, p);
 }

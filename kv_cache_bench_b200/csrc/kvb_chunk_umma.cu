@@ -54,6 +54,33 @@ constexpr int CU_FOLD_F32 = KVB_CHUNK_FOLD_F32, CU_FOLD_F16 = KVB_CHUNK_FOLD_F16
 constexpr float CU_SHIFT = 5.f;  // a row's highest score so far has probability 2^CU_SHIFT: small ones stay normal in fp16
 constexpr float CU_MOST = 16384.f;  // a key tile's probabilities of a row may sum to this before the reference moves
 
+// The work of a call is a line: sequence by sequence, KV head by KV head, unit by unit, each unit as long as
+// its cost (keys, and an overhead), cut into equal parts, one per CTA. So every CTA ends at about the same
+// time whatever the lengths, and a call with few units splits their keys. A unit that a cut goes through
+// (at a key tile) is computed in pieces, which a second small kernel joins. Costs are in quarter keys: a
+// unit with one query tile counts three quarters.
+constexpr long long CU_COST_UNIT = 4 * 480;       // a unit's overhead
+constexpr long long CU_COST_LEAST = 4 * 512;      // work that is worth a CTA
+constexpr int CU_SNAP = 2;                        // no cut nearer than this to a unit's first or last key tile
+
+// The first k units of a sequence (of one KV head) on that line.
+__device__ __forceinline__ long long cost_upto(const ChunkParams& p, const ChunkSeq& s, long long k) {
+    if (s.bad) return k * CU_COST_UNIT;
+    if (s.n <= p.tile_tokens) return k * (CU_COST_UNIT + 3ll * (s.ctx + s.n));
+    return k * (CU_COST_UNIT + 4ll * s.ctx) + 2ll * p.unit_tokens * k * (k + 1);
+}
+__device__ __forceinline__ int seq_units(const ChunkParams& p, const ChunkSeq& s) {
+    return s.bad ? 1 : (s.n + p.unit_tokens - 1) / p.unit_tokens;
+}
+
+// Where the cut at x of a unit of cost w falls among its nt key tiles.
+__device__ __forceinline__ int cut_tile(long long x, long long w, int nt) {
+    if (x <= 0) return 0;
+    if (x >= w) return nt;
+    const int k = int(x * nt / w);
+    return k < CU_SNAP ? 0 : k > nt - CU_SNAP ? nt : k;
+}
+
 template <int SRC, bool QF32, int D>
 struct CCfg {
     static constexpr int NSUB = D / 64;
@@ -98,6 +125,7 @@ struct RingUnit {
     ChunkUnit u;
     int t0;         // first key tile
     int nt[2];      // key tiles of the two query tiles
+    int slot;       // where its partial result goes; -1: the unit is whole
     int odd;        // a seen value was not finite (set by the cleaning warps)
     int bad;        // a block id was refused (set by the producer)
 };
@@ -230,6 +258,58 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
     pdl_wait();
     pdl_trigger();
 
+    // This CTA's part of the work: the whole line's length (every thread adds up some sequences), then the
+    // sequence that the part begins in. The sums use the stages' memory, which nothing loads into yet.
+    long long* s_sum = reinterpret_cast<long long*>(smem + C::KV_OFF);
+    volatile long long* s_begin = s_sum + C::THREADS;  // sequence, place in it
+    const int per = (p.B + C::THREADS - 1) / C::THREADS;
+    const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+    auto seq_cost = [&](int b) {
+        const ChunkSeq s = chunk_seq(p, b);
+        return p.Hkv * cost_upto(p, s, seq_units(p, s));
+    };
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += seq_cost(b);
+    s_sum[tid] = mine;
+    if (tid == 0) s_begin[0] = p.B;
+    __syncthreads();
+    if (warp == 0) {  // exclusive sums, and the total behind them
+        long long carry = 0;
+        for (int i = lane; i < C::THREADS; i += 32) {
+            const long long v = s_sum[i];
+            long long x = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            s_sum[i] = carry + x - v;
+            carry += __shfl_sync(0xffffffffu, x, 31);
+        }
+        if (lane == 0) s_begin[2] = carry;
+    }
+    __syncthreads();
+    const long long line = s_begin[2];
+    const long long parts = min((long long)p.ctas, max(1ll, line / CU_COST_LEAST));
+    auto part_begin = [&](long long c) { return c >= parts ? line : line * c / parts; };
+    const long long my_begin = part_begin(blockIdx.x), my_end = part_begin(blockIdx.x + 1ll);
+    if (my_begin < my_end && s_sum[tid] <= my_begin && my_begin < s_sum[tid] + mine) {
+        long long at = my_begin - s_sum[tid];
+        int b = b0;
+        for (; b < b1; ++b) {
+            const long long w = seq_cost(b);
+            if (at < w) break;
+            at -= w;
+        }
+        s_begin[0] = b;
+        s_begin[1] = at;
+    }
+    __syncthreads();
+    const int first_seq = int(s_begin[0]);
+    const long long first_at = s_begin[1];
+    fence_proxy_async_smem();
+    __syncthreads();  // read before the stages are loaded
+
     // False once a wait has given up (here, or elsewhere in the CTA where this one would block).
     auto wait = [&](uint64_t* bar, uint32_t parity) {
         if (mbar_try_wait(bar, parity & 1)) return true;
@@ -258,7 +338,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             if (stop()) break;
             const RingUnit& R = ring(e);
             const ChunkUnit u = R.u;
-            const int nt = R.nt[t], nall = max(R.nt[0], R.nt[1]), kt0 = R.t0;
+            const int nt = R.nt[t], nall = max(R.nt[0], R.nt[1]), kt0 = R.t0, slot = R.slot;
             if (u.state < 0) break;
             auto leave = [&]() {
                 __syncwarp();
@@ -500,10 +580,10 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             const volatile RingUnit& V = R;
             const bool bad = V.bad != 0, odd = V.odd != 0;
             if (bad && r == 0) raise_error(p.error_flag, KVB_DEVERR_BLOCK);
-            float inv = bad ? __int_as_float(0x7fc00000) : p.splits > 1 && l == 0.f ? 0.f : 1.f / l;
+            float inv = bad ? __int_as_float(0x7fc00000) : slot >= 0 && l == 0.f ? 0.f : 1.f / l;
             const size_t row = (size_t)qrow * p.H + h;
-            const size_t at = (size_t)u.split * p.T * p.H + row;
-            if (p.splits > 1 && live) p.part_ml[at] = make_float2(ref, bad ? inv : l);
+            const size_t at = ((size_t)slot * 2 + t) * CU_ROWS + r;
+            if (slot >= 0 && live) p.part_ml[at] = make_float2(ref, bad ? inv : l);
             if constexpr (SRC == SRC_I8) inv = vexp != 0.f ? inv / vexp : inv;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
@@ -540,8 +620,8 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
                 if (!live) {
                     // a row of no token: nothing to store
-                } else if (QF32 || p.splits > 1) {
-                    uint4* out = reinterpret_cast<uint4*>(p.splits > 1 ? p.part_o + at * D + c
+                } else if (QF32 || slot >= 0) {
+                    uint4* out = reinterpret_cast<uint4*>(slot >= 0 ? p.part_o + at * D + c
                                                                        : static_cast<float*>(p.out) + row * D + c);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) out[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
@@ -561,45 +641,94 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
         reg_dealloc<C::REGS_REST>();
         if (warp == C::SOFT) {
             // ------------------------------------------------------------ producer and scheduler
-            const uint64_t policy = l2_evict_first_policy();
-            uint32_t item = 0, tiles = 0, units = 0;
+            uint32_t item = 0, tiles = 0, published = 0;
             uint32_t qn = 0;  // units whose queries were loaded
             uint32_t dirty_n = 0;  // value tiles sent to the cleaning warps
-            long long idx = blockIdx.x;
-            auto next = [&]() {
-                long long i = p.units;
-                if (p.next_unit && lane == 0) i = (long long)gridDim.x + atomicAdd(p.next_unit, 1u);
-                return p.next_unit ? __shfl_sync(0xffffffffu, i, 0) : i;
-            };
-            auto publish = [&](const ChunkUnit& u, int2 range, int nt0, int nt1) {
-                if (units >= CU_RING) wait(&r_empty[units % CU_RING], units / CU_RING - 1);
+            auto publish = [&](const ChunkUnit& u, int2 range, int nt0, int nt1, int slot) {
+                if (published >= CU_RING) wait(&r_empty[published % CU_RING], published / CU_RING - 1);
                 __syncwarp();
                 if (lane == 0) {
-                    RingUnit& R = ring(units);
+                    RingUnit& R = ring(published);
                     R.u = u;
                     R.t0 = range.x;
                     R.nt[0] = nt0;
                     R.nt[1] = nt1;
+                    R.slot = slot;
                     R.odd = R.bad = 0;
-                    mbar_arrive(&r_full[units % CU_RING]);
+                    mbar_arrive(&r_full[published % CU_RING]);
                 }
-                ++units;
+                ++published;
             };
-            for (; idx < p.units && !stop(); idx = next()) {
-                const ChunkUnit u = chunk_unit(p, idx);
-                if (u.state == 1) continue;
-                if (u.state == 2) {
-                    publish(u, make_int2(0, 0), 0, 0);
+            ChunkPiece piece{0, 0, 0, -1, 0};
+            long long place = my_begin, at = first_at;  // on the line; in the sequence
+            ChunkSeq s{};
+            int units = 0;
+            long long w = 0;  // cost of one KV head of sequence b
+            for (int b = first_seq, known = -1; b < p.B && place < my_end && !stop();) {
+                if (b != known) {
+                    known = b;
+                    s = chunk_seq(p, b);
+                    units = seq_units(p, s);
+                    w = cost_upto(p, s, units);
+                }
+                if (at >= w * p.Hkv) {
+                    at = 0;
+                    ++b;
                     continue;
                 }
-                const int2 range = chunk_split_tiles(p, u, CU_ROWS);
+                ChunkUnit u;
+                u.b = b;
+                u.kvh = int(at / w);
+                const long long x = at - u.kvh * w;
+                int k = 0, hi = units - 1;  // the unit: the last one that begins at or before x
+                while (k < hi) {
+                    const int mid = k + (hi - k + 1) / 2;
+                    if (cost_upto(p, s, mid) <= x) k = mid;
+                    else hi = mid - 1;
+                }
+                const long long u0 = cost_upto(p, s, k), uw = cost_upto(p, s, k + 1) - u0;
+                const long long xa = x - u0, xb = min(uw, xa + (my_end - place));  // this CTA's part of the unit
+                const long long unit_end = place + (uw - xa);
+                place += xb - xa;
+                at += xb - xa;
+                u.split = 0;
+                u.kv0 = s.c0;
+                if (s.bad) {
+                    u.state = 2;
+                    u.row0 = s.c0;
+                    u.n = s.n;
+                    u.pos0 = u.keys = 0;
+                    if (xa == 0) publish(u, make_int2(0, 0), 0, 0, -1);
+                    continue;
+                }
+                u.state = 0;
+                u.row0 = s.c0 + k * p.unit_tokens;
+                u.n = min(p.unit_tokens, s.n - k * p.unit_tokens);
+                u.pos0 = s.ctx + k * p.unit_tokens;
+                u.keys = u.pos0 + u.n;
+                const int nt_all = (u.keys + CU_ROWS - 1) / CU_ROWS;
+                const int2 range = make_int2(cut_tile(xa, uw, nt_all), cut_tile(xb, uw, nt_all));
+                if (range.x == range.y) continue;
+                int slot = -1;
+                if (range.x > 0) {
+                    slot = 2 * blockIdx.x;
+                    piece.head = 1;
+                } else if (range.y < nt_all) {
+                    slot = 2 * blockIdx.x + 1;
+                    piece.kvh = u.kvh;
+                    piece.row0 = u.row0;
+                    piece.n = u.n;
+                    long long c = blockIdx.x + 1;  // the last part that begins before the unit's end
+                    while (c + 1 < parts && part_begin(c + 1) < unit_end) ++c;
+                    piece.last = int(c);
+                }
                 const int n1 = u.n - p.tile_tokens;  // tokens of tile 1
                 const int keys0 = u.pos0 + min(u.n, p.tile_tokens);
                 const int nt0 = max(0, min(range.y, (keys0 + CU_ROWS - 1) / CU_ROWS) - range.x);
                 const int nt1 = n1 > 0 ? range.y - range.x : 0;
                 const int dirty = (u.pos0 + 1) / CU_ROWS - range.x;  // values from this tile on pass the cleaning warps
-                const int e = units;
-                publish(u, range, nt0, nt1);
+                const int e = published;
+                publish(u, range, nt0, nt1, slot);
                 const int nj = max(nt0, nt1);
                 if (nj == 0) continue;
                 const int bt = SRC == SRC_PACKED ? CU_ROWS : min(p.page, CU_ROWS);  // keys of a box
@@ -689,7 +818,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                                 const int y = (id * p.Hkv + u.kvh) * p.page + k % p.page;
 #pragma unroll
                                 for (int s = 0; s < NSUB; ++s)
-                                    tma_load_2d(dst + s * CU_SUB + lane * bt * 128, map, done, 64 * s, y, policy);
+                                    tma_load_2d(dst + s * CU_SUB + lane * bt * 128, map, done, 64 * s, y);
                             }
                         }
                     }
@@ -716,7 +845,8 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             }
             ChunkUnit end{};
             end.state = -1;
-            publish(end, make_int2(0, 0), 0, 0);
+            publish(end, make_int2(0, 0), 0, 0, -1);
+            if (lane == 0) p.pieces[blockIdx.x] = piece;
         } else if (warp == C::SOFT + 1 || (warp == C::SOFT + 2 && !C::ALIAS)) {
             // ------------------------------------------------------------ products
             if (tc_elect()) {
@@ -924,7 +1054,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
 
 template <int SRC, bool QF32, int D>
 cudaError_t launch(const ChunkParams& p, const CUtensorMap* tq, const CUtensorMap* tk, const CUtensorMap* tv,
-                   int num_sms, cudaStream_t stream) {
+                   cudaStream_t stream) {
     using C = CCfg<SRC, QF32, D>;
     static KvbPerDevice<int> configured;
     int done = 0;
@@ -934,19 +1064,13 @@ cudaError_t launch(const ChunkParams& p, const CUtensorMap* tq, const CUtensorMa
                                     int(C::SMEM));
     });
     if (e != cudaSuccess) return e;
-    const long long grid = std::min<long long>(p.units, num_sms);
-    if (p.next_unit) {
-        e = cudaMemsetAsync(p.next_unit, 0, sizeof(unsigned), stream);
-        if (e != cudaSuccess) return e;
-    }
-    return kvb_launch_pdl(chunk_umma_kernel<SRC, QF32, D>, (unsigned)grid, C::THREADS, C::SMEM, stream, *tq, *tk, *tv, p);
+    return kvb_launch_pdl(chunk_umma_kernel<SRC, QF32, D>, (unsigned)p.ctas, C::THREADS, C::SMEM, stream, *tq, *tk, *tv, p);
 }
 
 template <int SRC, bool QF32>
 cudaError_t launch_d(const ChunkParams& p, int D, const CUtensorMap* tq, const CUtensorMap* tk, const CUtensorMap* tv,
-                     int num_sms, cudaStream_t stream) {
-    return D == 128 ? launch<SRC, QF32, 128>(p, tq, tk, tv, num_sms, stream)
-                    : launch<SRC, QF32, 64>(p, tq, tk, tv, num_sms, stream);
+                     cudaStream_t stream) {
+    return D == 128 ? launch<SRC, QF32, 128>(p, tq, tk, tv, stream) : launch<SRC, QF32, 64>(p, tq, tk, tv, stream);
 }
 
 }  // namespace
@@ -961,14 +1085,14 @@ bool kvb_chunk_umma_supported(int q_type, int kv_type, bool paged, int D, int pa
 }
 
 cudaError_t kvb_launch_chunk_umma(const ChunkParams& p, int q_type, int kv_type, int D, const void* tmap_q,
-                                  const void* tmap_k, const void* tmap_v, int num_sms, cudaStream_t stream) {
+                                  const void* tmap_k, const void* tmap_v, cudaStream_t stream) {
     const CUtensorMap* tq = static_cast<const CUtensorMap*>(tmap_q);
     const CUtensorMap* tk = static_cast<const CUtensorMap*>(tmap_k);
     const CUtensorMap* tv = static_cast<const CUtensorMap*>(tmap_v);
-    if (!p.block_table) return launch_d<SRC_PACKED, false>(p, D, tq, tk, tv, num_sms, stream);
+    if (!p.block_table) return launch_d<SRC_PACKED, false>(p, D, tq, tk, tv, stream);
     if (kv_type == KVB_F16)
-        return q_type == KVB_F32 ? launch_d<SRC_F16, true>(p, D, tq, tk, tv, num_sms, stream)
-                                 : launch_d<SRC_F16, false>(p, D, tq, tk, tv, num_sms, stream);
-    return q_type == KVB_F32 ? launch_d<SRC_I8, true>(p, D, tq, tk, tv, num_sms, stream)
-                             : launch_d<SRC_I8, false>(p, D, tq, tk, tv, num_sms, stream);
+        return q_type == KVB_F32 ? launch_d<SRC_F16, true>(p, D, tq, tk, tv, stream)
+                                 : launch_d<SRC_F16, false>(p, D, tq, tk, tv, stream);
+    return q_type == KVB_F32 ? launch_d<SRC_I8, true>(p, D, tq, tk, tv, stream)
+                             : launch_d<SRC_I8, false>(p, D, tq, tk, tv, stream);
 }

@@ -39,7 +39,7 @@ struct Attend {
     int q_type, kv_type, kernel;
     bool paged;
     ChunkParams p;
-    int64_t workspace, fold_off;
+    int64_t workspace, pieces_off, ml_off, o_off, fold_off;  // bytes, and where in them
     bool umma;
 };
 
@@ -79,19 +79,29 @@ int geometry(Attend& a) {
     p.unit_tokens = a.umma ? 2 * p.tile_tokens : p.tile_tokens;
     p.blocks_of_new = (std::max(p.max_new, 1) + p.unit_tokens - 1) / p.unit_tokens;
     const long long base = (long long)p.blocks_of_new * p.B * p.Hkv;
-    const long long slots = a.umma ? sms : 2ll * sms, least = a.umma ? 512 : 128;  // CTAs that run at once, keys worth a part
+    const int64_t head = 256, D = s.head_dim;
+    a.workspace = head;
     p.splits = 1;
+    if (a.umma) {
+        // CTAs that share the work: an SM each, no more than parts of 512 keys of the longest sequences
+        const long long most = base * std::max<long long>(1, ((long long)p.max_len + 511) / 512);
+        p.ctas = (int)std::min<long long>(most, sms);
+        const int fold = a.q_type == KVB_F32 ? KVB_CHUNK_FOLD_F32 : KVB_CHUNK_FOLD_F16;
+        a.pieces_off = a.workspace;
+        a.ml_off = (int64_t)kvb_align_up(a.pieces_off + sizeof(ChunkPiece) * p.ctas, 256);
+        a.o_off = a.ml_off + (int64_t)sizeof(float2) * p.ctas * 2 * 256;
+        a.fold_off = a.o_off + 4 * D * p.ctas * 2 * 256;
+        a.workspace = a.fold_off + (p.max_len > fold * 128 ? 4 * D * p.ctas * 256 : 0);
+        return KVB_OK;
+    }
+    const long long slots = 2ll * sms, least = 128;  // CTAs that run at once, keys worth a part
     if (base < slots)
         p.splits = (int)std::max<long long>(1, std::min(slots / std::max<long long>(base, 1), p.max_len / least));
     p.units = base * p.splits;
     if (p.units >= (1ll << 31)) return invalid("more than 2^31 work units");
-    a.workspace = 256;
-    if (p.splits > 1) a.workspace += (long long)p.splits * p.T * p.H * (s.head_dim + 2) * 4 + 256;
-    a.workspace = (int64_t)kvb_align_up((size_t)a.workspace, 256);
-    a.fold_off = a.workspace;
-    const int fold = a.q_type == KVB_F32 ? KVB_CHUNK_FOLD_F32 : KVB_CHUNK_FOLD_F16;
-    if (a.umma && p.max_len > fold * 128)
-        a.workspace += std::min<long long>(p.units, sms) * 2 * 128 * s.head_dim * 4;
+    a.ml_off = head;
+    a.o_off = (int64_t)kvb_align_up(head + sizeof(float2) * (size_t)p.splits * p.T * p.H, 256);
+    if (p.splits > 1) a.workspace = a.o_off + 4 * D * p.splits * p.T * p.H;
     return KVB_OK;
 }
 
@@ -134,19 +144,20 @@ int run(Attend& a, void* workspace, size_t workspace_bytes, void* stream) {
     int sms = 0;
     if (int rc = kvb_device_sms(&sms)) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    p.next_unit = a.umma && p.units > sms ? static_cast<unsigned*>(workspace) : nullptr;
-    p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + 256);
-    p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                        kvb_align_up(256 + sizeof(float2) * (size_t)p.splits * p.T * p.H, 256));
-    p.fold = reinterpret_cast<float*>(static_cast<char*>(workspace) + a.fold_off);
+    char* ws = static_cast<char*>(workspace);
+    p.pieces = reinterpret_cast<ChunkPiece*>(ws + a.pieces_off);
+    p.part_ml = reinterpret_cast<float2*>(ws + a.ml_off);
+    p.part_o = reinterpret_cast<float*>(ws + a.o_off);
+    p.fold = reinterpret_cast<float*>(ws + a.fold_off);
     cudaError_t e;
     if (a.umma) {
         CUtensorMap tq, tk, tv;
         if (int rc = tensor_maps(a, &tq, &tk, &tv)) return rc;
-        e = kvb_launch_chunk_umma(p, a.q_type, a.kv_type, a.s.head_dim, &tq, &tk, &tv, sms, st);
-    } else {
-        e = kvb_launch_chunk_simt(p, a.q_type, a.kv_type, a.s.head_dim, st);
+        e = kvb_launch_chunk_umma(p, a.q_type, a.kv_type, a.s.head_dim, &tq, &tk, &tv, st);
+        if (e == cudaSuccess && p.ctas > 1) e = kvb_launch_chunk_join(p, a.q_type, a.s.head_dim, st);
+        return launched(e);
     }
+    e = kvb_launch_chunk_simt(p, a.q_type, a.kv_type, a.s.head_dim, st);
     if (e == cudaSuccess && p.splits > 1) e = kvb_launch_chunk_merge(p, a.q_type, a.s.head_dim, sms, st);
     return launched(e);
 }

@@ -68,6 +68,21 @@ def test_chunk_many_units(qt, kv):
     run_chunk([n + i for i in range(6)], [90 * i for i in range(6)], 32, 16, 64, 16, qt, kv)
 
 
+@pytest.mark.parametrize("qt,kv", TYPES)
+@pytest.mark.parametrize("B", [500, 1300])
+def test_chunk_many_sequences(qt, kv, B):
+    # more sequences than a CTA has threads, some without new tokens
+    new = [i % 4 for i in range(B)]
+    ctx = [(7 * i) % 90 + (2000 if i % 97 == 0 else 0) for i in range(B)]
+    run_chunk(new, ctx, 4, 2, 64, 16, qt, kv)
+
+
+@pytest.mark.parametrize("qt,kv", [(F16, F16), (F32, F16), (F16, I8), (F32, I8)])
+def test_chunk_long_keys_few_ctas(qt, kv):
+    # so many units that each CTA takes long runs of key tiles: the running sums leave tensor memory
+    run_chunk([256, 250], [20000, 9000], 32, 32, 64, 128, qt, kv)
+
+
 @pytest.mark.parametrize("qt", [F16, F32])
 def test_chunk_query_stride(qt):
     run_chunk([20, 7], [40, 0], 8, 2, 128, 16, qt, F16, pad=64)
