@@ -8,25 +8,19 @@
 //     P = exp2(f S - m), l += row sums
 //     O[128 rows x D] += P V              (P in tensor memory over S, V in shared memory, MN-major)
 // with the running reference m of a row raised only when a score passes it by 2^8 (then O and l are
-// scaled in place), so O stays in tensor memory. One persistent CTA per SM:
-//   warps 0-15      softmax: eight warps per query tile, a thread per row (tensor-memory lane) and half of
-//                   the key tile. While one tile's warps compute, the products of the other run; four
-//                   compute warps per scheduler hide each other's latencies (with two, a key tile took
-//                   2700 cycles of softmax instead of about 1400, the same instructions). Probabilities are
-//                   computed with the reference so far and the maximum beside them; only if a score passes
-//                   the reference are they computed again.
-//   warp 16         TMA producer and unit scheduler: K and V tiles into a ring of stages, Q tiles, and
-//                   the units (first blockIdx.x, then one at a time from a counter) through a small ring.
-//   warps 17, 18    one elected thread each issues the score products and the value products. (A lane
-//                   chosen by its number instead of elect.sync took 85 cycles a product, longer than the
-//                   product, and one thread for both kinds was the bottleneck: with its share of waits and
-//                   commits it took 2000 cycles a key tile and query tile, twice the products' time.) With
-//                   split operands (QF32) a tile's scores and probabilities share their columns, and one
-//                   thread issues both kinds in order.
-//   warp 19         fp16 values: non-finite elements of tiles that some row does not see in full are set
-//                   to 0 (0 x inf would not be 0) and, where a row does see them, added at the end.
-//   warps 20-23     int8: tiles converted to fp16 (exact), the scales are applied to the scores and to the
-//                   probabilities.
+// scaled in place), so O stays in tensor memory. One persistent CTA per SM, 16 warps:
+//   0-3, 4-7   softmax of query tiles 0 and 1, one thread per row (tensor-memory lane).
+//   8          unit scheduler, and TMA producer of the key tiles and the query tiles.
+//   9          TMA producer of the value tiles (with small pages one warp's issue of 16 boxes a tile was slower
+//              than the memory).
+//   10, 11     one elected thread each issues the score products and the value products. (A lane chosen by
+//              its number instead of elect.sync took 85 cycles a product, longer than the product, and one
+//              thread for both kinds was the bottleneck: with its share of waits and commits it took 2000
+//              cycles a key tile and query tile, twice the products' time.) With split operands (QF32) a
+//              tile's scores and probabilities share their columns, and warp 10 issues both kinds in order.
+//   12-15      fp16 values: non-finite elements of tiles that some row does not see in full are set to 0
+//              (0 x inf would not be 0) and, where a row does see them, added at the end. int8: tiles
+//              converted to fp16 (exact); the scales are applied to the scores and to the probabilities.
 // fp32 queries (QF32) keep fp32-level results: q and p are split as fp16(x) + fp16(x - fp16(x)) (about 22
 // bits; q prescaled per row by a power of two) and both products run on both halves.
 #include <cuda.h>
@@ -45,7 +39,7 @@ constexpr int CU_ROWS = 128;            // query rows of a tile, keys of a tile
 constexpr int CU_SUB = CU_ROWS * 128;   // bytes of [128 rows][128 B], one 128-byte-swizzled slice
 constexpr int CU_RING = 2;              // units in flight between the roles
 constexpr int CU_POLY = 0, CU_POLY_OF = 4;  // pairs of probabilities on the FMA pipe, of so many
-constexpr int CU_CLEAN = 4;             // value tiles on their way to the cleaning warps: at most three are
+constexpr int CU_CLEAN = 8;             // value tiles on their way to the cleaning warps: at most their stages are
 enum { SRC_F16 = 0, SRC_I8 = 1, SRC_PACKED = 2 };
 // The tensor cores add into O with truncation, an error of up to 2^-23 of O per product of 16 keys and in
 // one direction. So O is added into an fp32 sum in the workspace (rounded to nearest) and started anew
@@ -88,16 +82,17 @@ struct CCfg {
     static constexpr int QTILE = NSUB * CU_SUB * (QF32 ? 2 : 1);
     static constexpr int RAW = CU_ROWS * D;                 // one int8 tile
     static constexpr int BUDGET = 227 * 1024 - 1024 - 2048;  // alignment, small arrays
-    static constexpr int NR = SRC == SRC_I8 ? (QF32 ? 2 : 3) : 0;
-    static constexpr int FIT = (BUDGET - 2 * QTILE - NR * RAW) / ITEM;
-    static constexpr int NS = FIT > 6 - NR ? 6 - NR : FIT;  // int8: at most six items in flight (scale ring)
-    static constexpr int SOFT = 8;                          // softmax warps
-    static constexpr int HELPERS = SRC == SRC_I8 ? 4 : 1;   // converting or cleaning warps
-    static constexpr int HELPER0 = SOFT + (SRC == SRC_I8 ? 4 : 3);
-    static constexpr int THREADS = 32 * (SOFT + (SRC == SRC_I8 ? 8 : 4));
+    // Stages of K and of V: int8 tiles as loaded, fp16 tiles. (int8: few enough that the scales of SR key
+    // tiles cover those on their way.)
+    static constexpr int RAWS = SRC != SRC_I8 ? 0 : QF32 && D == 128 ? 1 : 2;
+    static constexpr int FIT = (BUDGET - 2 * QTILE - 2 * RAWS * RAW) / ITEM;
+    static constexpr int MOST = SRC == SRC_I8 ? 6 : CU_CLEAN;
+    static constexpr int STAGES = FIT > MOST ? MOST : FIT;
+    static constexpr int NK = STAGES / 2, NV = STAGES - NK;
+    static constexpr int SOFT = 8, HELPER0 = 12, HELPERS = 4, THREADS = 512;
     // registers per thread after the split; the launch gives 65536 / THREADS, rounded down to 8
     static constexpr int REGS_LAUNCH = 65536 / THREADS / 8 * 8;
-    static constexpr int REGS_REST = SRC == SRC_I8 ? 80 : 88;
+    static constexpr int REGS_REST = 64;
     static constexpr int REGS_SOFT = (THREADS * REGS_LAUNCH - (THREADS - 32 * SOFT) * REGS_REST) / (32 * SOFT) / 8 * 8;
     // Tensor-memory columns. fp16 probabilities have their own, so that a tile's next scores need not wait
     // for its value product; split ones lie over their scores. O of tile t is at O_COL + D t.
@@ -105,18 +100,21 @@ struct CCfg {
     static constexpr int SBUFS = ALIAS || D == 64 ? 2 : 1;    // score buffers: the tiles', or one that they share
     static constexpr int O_COL = ALIAS ? 256 : 128 * SBUFS + 128;
     static_assert(O_COL + 2 * D <= 512, "tensor memory");
-    static constexpr int SR = ALIAS ? 4 : 8;                  // int8: key tiles whose scales are kept
+    // int8: key tiles whose scales are kept. A tile's are written when the keys RAWS + NK tiles before it are
+    // through their score products; a softmax may then still be reading those of the tile before.
+    static constexpr int SR = QF32 && D == 128 ? 4 : 8;
+    static_assert(RAWS + NK + 2 <= SR, "scale ring");
     static constexpr size_t Q_OFF = 0;
     static constexpr size_t KV_OFF = 2 * QTILE;
-    static constexpr size_t RAW_OFF = KV_OFF + size_t(NS) * ITEM;
-    static constexpr size_t BAR_OFF = RAW_OFF + size_t(NR) * RAW;
-    static constexpr int NBARS = 2 * NS + 2 * NR + 11 + CU_CLEAN + 2 * CU_RING;
+    static constexpr size_t RAW_OFF = KV_OFF + size_t(STAGES) * ITEM;  // (K's stages, then V's)
+    static constexpr size_t BAR_OFF = RAW_OFF + size_t(2 * RAWS) * RAW;
+    static constexpr int NBARS = 2 * STAGES + 4 * RAWS + 11 + CU_CLEAN + 2 * CU_RING;
     static constexpr size_t UNIT_OFF = kvb_align_up(BAR_OFF + 8 * NBARS, 64);
     static constexpr size_t SCALE_OFF = UNIT_OFF + 64 * CU_RING;           // [SR tiles][K, V][16 pages]
-    static constexpr size_t VMAX_OFF = SCALE_OFF + (NR ? SR * 2 * 16 * 4 : 0);  // [SR tiles]
-    static constexpr size_t MISC_OFF = kvb_align_up(VMAX_OFF + (NR ? SR * 4 : 0), 16);
-    static constexpr size_t SMEM = MISC_OFF + 16 + 1024;
-    static_assert(NS >= 2 && SMEM <= 227 * 1024, "shared memory budget");
+    static constexpr size_t VMAX_OFF = SCALE_OFF + (RAWS ? SR * 2 * 16 * 4 : 0);  // [SR tiles]
+    static constexpr size_t MISC_OFF = kvb_align_up(VMAX_OFF + (RAWS ? SR * 4 : 0), 16);
+    static constexpr size_t SMEM = MISC_OFF + 16 + 4 * CU_CLEAN + 1024;
+    static_assert(NK >= 1 && NV >= 1 && SMEM <= 227 * 1024, "shared memory budget");
     static_assert(KV_OFF % 1024 == 0 && RAW_OFF % 1024 == 0, "swizzled tiles need 1024-byte alignment");
 };
 
@@ -209,15 +207,20 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                       const __grid_constant__ CUtensorMap tmv, const __grid_constant__ ChunkParams p) {
     using C = CCfg<SRC, QF32, D>;
     using QT = typename std::conditional<QF32, float, __half>::type;
-    constexpr int NSUB = C::NSUB, NS = C::NS;
+    constexpr int NSUB = C::NSUB, NK = C::NK, NV = C::NV, RAWS = C::RAWS;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_u32(smem);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);  // [NS] K or V tile ready for the products
-    uint64_t* empty = full + NS;         // [NS] its products are done
-    uint64_t* raw_full = empty + NS;     // [NR] int8 tile loaded
-    uint64_t* raw_empty = raw_full + C::NR;
-    uint64_t* q_full = raw_empty + C::NR;  // [2] query tile in shared memory
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+    uint64_t* k_full = bars;             // [NK] key tile ready for the products
+    uint64_t* v_full = k_full + NK;      // [NV] value tile ready
+    uint64_t* k_empty = v_full + NV;     // [NK] its products are done
+    uint64_t* v_empty = k_empty + NK;
+    uint64_t* rk_full = v_empty + NV;    // [RAWS] int8 key tile loaded
+    uint64_t* rv_full = rk_full + RAWS;
+    uint64_t* rk_empty = rv_full + RAWS;  // [RAWS] ... and converted
+    uint64_t* rv_empty = rk_empty + RAWS;
+    uint64_t* q_full = rv_empty + RAWS;  // [2] query tile in shared memory
     uint64_t* q_empty = q_full + 2;      // both query tiles' score products are done
     uint64_t* s_full = q_empty + 1;      // [2] scores of the tile ready
     uint64_t* s_free = s_full + 2;       // [SBUFS] scores read into registers (not with ALIAS)
@@ -231,23 +234,27 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
     float* s_vmax = reinterpret_cast<float*>(smem + C::VMAX_OFF);
     volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::MISC_OFF);
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::MISC_OFF + 8);
+    unsigned* s_clean = reinterpret_cast<unsigned*>(smem + C::MISC_OFF + 16);  // [CU_CLEAN] cleaning warps done
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (warp == 0) {
         for (int i = lane; i < C::NBARS; i += 32) {
-            uint64_t* b = full + i;
+            uint64_t* b = bars + i;
             uint32_t n = 1;
-            if (b < empty) n = SRC == SRC_I8 ? C::HELPERS : 1;
-            else if (b >= raw_empty && b < q_full) n = C::HELPERS;
+            if (b < k_empty) n = SRC == SRC_I8 ? C::HELPERS / 2 : 1;
+            else if (b >= rk_empty && b < q_full) n = C::HELPERS / 2;
             else if (b >= q_full && b < q_empty) n = QF32 ? C::SOFT / 2 : 1;
             else if (b >= s_free && b < pv_done) n = C::SOFT / 2;
-            else if (b >= r_empty) n = (C::ALIAS ? 1 : 2) + C::SOFT + C::HELPERS;  // issuers, softmax warps, helpers
+            else if (b >= r_empty) n = (C::ALIAS ? 2 : 3) + C::SOFT + C::HELPERS;  // V producer, issuers, the rest
             mbar_init(b, n);
         }
-        if (lane == 0) *s_abort = 0;
+        if (lane == 0) {
+            *s_abort = 0;
+            for (int i = 0; i < CU_CLEAN; ++i) s_clean[i] = 0;
+        }
         fence_mbarrier_init();
     }
-    if (warp == C::SOFT + 1) {
+    if (warp == 10) {
         tc_alloc(s_tmem, 512);
         tc_relinquish();
     }
@@ -639,11 +646,54 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
         }
     } else {
         reg_dealloc<C::REGS_REST>();
-        if (warp == C::SOFT) {
-            // ------------------------------------------------------------ producer and scheduler
-            uint32_t item = 0, tiles = 0, published = 0;
-            uint32_t qn = 0;  // units whose queries were loaded
-            uint32_t dirty_n = 0;  // value tiles sent to the cleaning warps
+        // One K or V tile (key tile `tile` of unit u) into stage `st` of its kind, by a whole warp: this lane's
+        // box is page (or 128 tokens of a larger page) `id`.
+        const int bt = SRC == SRC_PACKED ? CU_ROWS : min(p.page, CU_ROWS);  // keys of a box
+        auto box_id = [&](const ChunkUnit& u, int tile, int end) {
+            const int k = tile * CU_ROWS + lane * bt;
+            if (SRC == SRC_PACKED || tile >= end || lane * bt >= CU_ROWS || k >= u.keys) return -1;
+            return __ldg(p.block_table + (size_t)u.b * p.max_blocks + k / p.page);
+        };
+        auto load_tile = [&](const ChunkUnit& u, int tile, int id, bool is_v, uint32_t st, uint64_t* done, RingUnit& R) {
+            const int k = tile * CU_ROWS + lane * bt;
+            const bool wanted = SRC != SRC_PACKED && lane * bt < CU_ROWS && k < u.keys;
+            const bool ok = wanted && id >= 0 && id < p.num_blocks;
+            if (__any_sync(0xffffffffu, wanted && !ok) && lane == 0) reinterpret_cast<volatile RingUnit&>(R).bad = 1;
+            const uint32_t boxes = SRC == SRC_PACKED ? 1 : __popc(__ballot_sync(0xffffffffu, ok));
+            const uint32_t bytes = SRC == SRC_I8 ? uint32_t(bt) * D : uint32_t(bt) * 128 * NSUB;  // of a box
+            const bool off = *s_abort != 0;
+            if (lane == 0) {
+                if (boxes && !off) mbar_arrive_expect_tx(done, boxes * bytes);
+                else mbar_arrive(done);
+            }
+            if (__any_sync(0xffffffffu, off)) return;  // (lane 0 may have expected bytes: the waits give up too)
+            if constexpr (SRC == SRC_I8) {
+                if (ok)
+                    bulk_load(smem + C::RAW_OFF + ((is_v ? RAWS : 0) + st) * C::RAW + lane * bytes,
+                              static_cast<const int8_t*>(is_v ? p.v : p.k) +
+                                  (((long long)id * p.Hkv + u.kvh) * p.page + k % p.page) * D,
+                              bytes, done);
+            } else {
+                uint8_t* dst = smem + C::KV_OFF + ((is_v ? NK : 0) + st) * C::ITEM;
+                const CUtensorMap* map = is_v ? &tmv : &tmk;
+                if constexpr (SRC == SRC_PACKED) {
+                    if (lane == 0)
+#pragma unroll
+                        for (int s = 0; s < NSUB; ++s)
+                            tma_load_3d(dst + s * CU_SUB, map, done, 64 * s, u.kvh, u.kv0 + tile * CU_ROWS);
+                } else if (ok) {
+                    const int y = (id * p.Hkv + u.kvh) * p.page + k % p.page;
+#pragma unroll
+                    for (int s = 0; s < NSUB; ++s)
+                        tma_load_2d(dst + s * CU_SUB + lane * bt * 128, map, done, 64 * s, y);
+                }
+            }
+            __syncwarp();
+        };
+        if (warp == 8) {
+            // ------------------------------------------------------------ scheduler, keys and queries
+            uint32_t item = 0, published = 0;  // key tiles, units
+            uint32_t qn = 0;                   // units whose queries were loaded
             auto publish = [&](const ChunkUnit& u, int2 range, int nt0, int nt1, int slot) {
                 if (published >= CU_RING) wait(&r_empty[published % CU_RING], published / CU_RING - 1);
                 __syncwarp();
@@ -726,104 +776,37 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 const int keys0 = u.pos0 + min(u.n, p.tile_tokens);
                 const int nt0 = max(0, min(range.y, (keys0 + CU_ROWS - 1) / CU_ROWS) - range.x);
                 const int nt1 = n1 > 0 ? range.y - range.x : 0;
-                const int dirty = (u.pos0 + 1) / CU_ROWS - range.x;  // values from this tile on pass the cleaning warps
                 const int e = published;
                 publish(u, range, nt0, nt1, slot);
                 const int nj = max(nt0, nt1);
                 if (nj == 0) continue;
-                const int bt = SRC == SRC_PACKED ? CU_ROWS : min(p.page, CU_ROWS);  // keys of a box
-                const int nbox = CU_ROWS / bt;
-                const int* table = p.block_table + (SRC == SRC_PACKED ? 0 : (size_t)u.b * p.max_blocks);
-                // Items: K of tile 0, then K of the next tile and V of this one in turn, V of the last tile:
-                // scores run a tile ahead of the values. The block id of this lane's box of a tile is read a
-                // tile ahead.
-                auto fetch = [&](int j) {
-                    const int k = (range.x + j) * CU_ROWS + lane * bt;
-                    return SRC != SRC_PACKED && j < nj && lane < nbox && k < u.keys ? __ldg(table + k / p.page) : -1;
-                };
-                int id_v = -1, id_k = fetch(0), id_n = fetch(1);  // of the value tile, the key tile, the next one
-                for (int i = 0; i < 2 * nj && !stop(); ++i) {
-                    const bool is_v = i == 2 * nj - 1 || (i > 0 && i % 2 == 0);
-                    const int j = is_v ? (i == 2 * nj - 1 ? nj - 1 : i / 2 - 1) : (i + 1) / 2;
-                    if (!is_v && i > 0) {
-                        id_v = id_k;
-                        id_k = id_n;
-                        id_n = fetch(j + 1);
-                    }
-                    if (i == 2 * nj - 1) id_v = id_k;
-                    const int id = is_v ? id_v : id_k;
-                    const int k = (range.x + j) * CU_ROWS + lane * bt;
-                    const bool wanted = SRC != SRC_PACKED && lane < nbox && k < u.keys;
-                    const bool ok = wanted && id >= 0 && id < p.num_blocks;
-                    if (!is_v && __any_sync(0xffffffffu, wanted && !ok) && lane == 0)
-                        reinterpret_cast<volatile RingUnit&>(ring(e)).bad = 1;
-                    const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, ok));
+                const int end_tile = range.x + nj;
+                int id = box_id(u, range.x, end_tile);  // read a tile ahead
+                for (int tile = range.x; tile < end_tile && !stop(); ++tile, ++item) {
+                    const int next = box_id(u, tile + 1, end_tile);
                     if constexpr (SRC == SRC_I8) {
-                        const uint32_t st = item % C::NR;
-                        float ks = 0.f, vs = 0.f;
-                        if (ok && !is_v) {
-                            ks = __ldg(p.k_scale + (long long)id * p.Hkv + u.kvh);
-                            vs = __ldg(p.v_scale + (long long)id * p.Hkv + u.kvh);
+                        const uint32_t st = item % RAWS;
+                        const bool ok = id >= 0 && id < p.num_blocks;
+                        const float ks = ok ? __ldg(p.k_scale + (long long)id * p.Hkv + u.kvh) : 0.f;
+                        const float vs = ok ? __ldg(p.v_scale + (long long)id * p.Hkv + u.kvh) : 0.f;
+                        if (item >= RAWS) wait(&rk_empty[st], item / RAWS - 1);
+                        // (the slot's readers are done: fewer than SR key tiles are on their way)
+                        const float vm = warp_max(vs <= 3.402823466e38f ? vs : 0.f);
+                        if (lane < 16) {
+                            s_scale[item % C::SR * 32 + lane] = ks;
+                            s_scale[item % C::SR * 32 + 16 + lane] = vs;
                         }
-                        if (item >= C::NR) wait(&raw_empty[st], item / C::NR - 1);
-                        if (!is_v) {
-                            // (the slot's readers are done: of the six items in flight at most, three are keys)
-                            const float vm = warp_max(vs <= 3.402823466e38f ? vs : 0.f);
-                            if (lane < 16) {
-                                s_scale[tiles % C::SR * 32 + lane] = ks;
-                                s_scale[tiles % C::SR * 32 + 16 + lane] = vs;
-                            }
-                            if (lane == 0) s_vmax[tiles % C::SR] = vm;
-                            ++tiles;
-                        }
+                        if (lane == 0) s_vmax[item % C::SR] = vm;
                         __syncwarp();
-                        const uint32_t bytes = uint32_t(bt) * D;
-                        if (lane == 0) {
-                            if (boxes && !*s_abort) mbar_arrive_expect_tx(&raw_full[st], boxes * bytes);
-                            else mbar_arrive(&raw_full[st]);
-                        }
-                        __syncwarp();
-                        if (ok && !*s_abort) {
-                            const int8_t* src = static_cast<const int8_t*>(is_v ? p.v : p.k) +
-                                                (((long long)id * p.Hkv + u.kvh) * p.page + k % p.page) * D;
-                            bulk_load(smem + C::RAW_OFF + st * C::RAW + lane * bytes, src, bytes, &raw_full[st]);
-                        }
+                        load_tile(u, tile, id, false, st, &rk_full[st], ring(e));
                     } else {
-                        const uint32_t st = item % NS;
-                        if (item >= NS) wait(&empty[st], item / NS - 1);
+                        const uint32_t st = item % NK;
+                        if (item >= NK) wait(&k_empty[st], item / NK - 1);
                         __syncwarp();
-                        uint8_t* dst = smem + C::KV_OFF + st * C::ITEM;
-                        const CUtensorMap* map = is_v ? &tmv : &tmk;
-                        uint64_t* done = &full[st];
-                        if (is_v && j >= dirty) done = &dirty_full[dirty_n++ % CU_CLEAN];
-                        if constexpr (SRC == SRC_PACKED) {
-                            if (lane == 0) {
-                                if (*s_abort) {
-                                    mbar_arrive(done);
-                                } else {
-                                    mbar_arrive_expect_tx(done, C::ITEM);
-#pragma unroll
-                                    for (int s = 0; s < NSUB; ++s)
-                                        tma_load_3d(dst + s * CU_SUB, map, done, 64 * s, u.kvh,
-                                                    u.kv0 + (range.x + j) * CU_ROWS);
-                                }
-                            }
-                        } else {
-                            if (lane == 0) {
-                                if (boxes && !*s_abort) mbar_arrive_expect_tx(done, boxes * bt * 128 * NSUB);
-                                else mbar_arrive(done);
-                            }
-                            __syncwarp();
-                            if (ok && !*s_abort) {
-                                const int y = (id * p.Hkv + u.kvh) * p.page + k % p.page;
-#pragma unroll
-                                for (int s = 0; s < NSUB; ++s)
-                                    tma_load_2d(dst + s * CU_SUB + lane * bt * 128, map, done, 64 * s, y);
-                            }
-                        }
+                        load_tile(u, tile, id, false, st, &k_full[st], ring(e));
                     }
-                    ++item;
-                    if (!QF32 && i == 0) {
+                    id = next;
+                    if (!QF32 && tile == range.x) {
                         // the queries, once the unit before has used its own
                         if (qn > 0) wait(q_empty, qn - 1);
                         ++qn;
@@ -847,7 +830,36 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             end.state = -1;
             publish(end, make_int2(0, 0), 0, 0, -1);
             if (lane == 0) p.pieces[blockIdx.x] = piece;
-        } else if (warp == C::SOFT + 1 || (warp == C::SOFT + 2 && !C::ALIAS)) {
+        } else if (warp == 9) {
+            // ------------------------------------------------------------ values
+            uint32_t item = 0, dirty_n = 0;  // value tiles, those that went to the cleaning warps
+            for (int e = 0; !stop(); ++e) {
+                wait(&r_full[e % CU_RING], e / CU_RING);
+                RingUnit& R = ring(e);
+                const ChunkUnit u = R.u;
+                if (u.state < 0) break;
+                const int end_tile = R.t0 + max(R.nt[0], R.nt[1]);
+                const int dirty = (u.pos0 + 1) / CU_ROWS;  // values from this tile on pass the cleaning warps
+                int tile = R.t0, id = box_id(u, tile, end_tile);
+                for (; tile < end_tile && !stop(); ++tile, ++item) {
+                    const int next = box_id(u, tile + 1, end_tile);
+                    if constexpr (SRC == SRC_I8) {
+                        const uint32_t st = item % RAWS;
+                        if (item >= RAWS) wait(&rv_empty[st], item / RAWS - 1);
+                        __syncwarp();
+                        load_tile(u, tile, id, true, st, &rv_full[st], R);
+                    } else {
+                        const uint32_t st = item % NV;
+                        if (item >= NV) wait(&v_empty[st], item / NV - 1);
+                        __syncwarp();
+                        load_tile(u, tile, id, true, st, tile >= dirty ? &dirty_full[dirty_n++ % CU_CLEAN] : &v_full[st], R);
+                    }
+                    id = next;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&r_empty[e % CU_RING]);
+            }
+        } else if (warp == 10 || (warp == 11 && !C::ALIAS)) {
             // ------------------------------------------------------------ products
             if (tc_elect()) {
                 constexpr uint32_t id_s = instr_desc(1, 0, 0, 0, 0, 128, 128);
@@ -855,9 +867,9 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 constexpr int FOLD = QF32 ? CU_FOLD_F32 : CU_FOLD_F16;
                 // descriptors of the first stage; a byte offset of o adds o / 16
                 const uint64_t kd = smem_desc(sbase + uint32_t(C::KV_OFF), 16, 1024);
-                const uint64_t vd = smem_desc(sbase + uint32_t(C::KV_OFF), CU_SUB, 1024);
+                const uint64_t vd = smem_desc(sbase + uint32_t(C::KV_OFF + NK * C::ITEM), CU_SUB, 1024);
                 const uint64_t qd = smem_desc(sbase + uint32_t(C::Q_OFF), 16, 1024);
-                uint32_t item = 0;                // first item of the unit
+                uint32_t item = 0;                // key tiles before the unit (and value tiles)
                 uint32_t nq0 = 0, nq1 = 0, np0 = 0, np1 = 0, nb0 = 0, nb1 = 0;  // uses of each barrier
                 auto scores = [&](int t, uint32_t it) {
                     if constexpr (!C::ALIAS) {  // the buffer's scores before these were read
@@ -866,7 +878,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                         ++nb;
                     }
                     tc_fence_after();
-                    const uint64_t k = kd + (it % NS) * (C::ITEM / 16), q = qd + t * (C::QTILE / 16);
+                    const uint64_t k = kd + (it % NK) * (C::ITEM / 16), q = qd + t * (C::QTILE / 16);
 #pragma unroll
                     for (int part = 0; part < (QF32 ? 2 : 1); ++part)
 #pragma unroll
@@ -877,7 +889,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     tc_commit(&s_full[t]);
                 };
                 auto values = [&](int t, uint32_t it, bool keep) {
-                    const uint64_t v = vd + (it % NS) * (C::ITEM / 16);
+                    const uint64_t v = vd + (it % NV) * (C::ITEM / 16);
                     const uint32_t tp = tmem + (C::ALIAS ? 128 * t : 128 * C::SBUFS + 64 * t), to = tmem + C::O_COL + D * t;
 #pragma unroll
                     for (int i = 0; i < CU_ROWS / 16; ++i) {
@@ -892,7 +904,8 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     }
                     tc_commit(&pv_done[t]);
                 };
-                auto ready = [&](uint32_t it) { return wait(&full[it % NS], it / NS); };
+                auto keys_ready = [&](uint32_t it) { return wait(&k_full[it % NK], it / NK); };
+                auto values_ready = [&](uint32_t it) { return wait(&v_full[it % NV], it / NV); };
                 for (int e = 0; !*s_abort; ++e) {
                     wait(&r_full[e % CU_RING], e / CU_RING);
                     const RingUnit& R = ring(e);
@@ -901,45 +914,43 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     if (state < 0) break;
                     const int nj = max(nt0, nt1);
                     if (nj == 0) continue;
-                    auto key_item = [&](int j) { return item + (j == 0 ? 0 : 2 * j - 1); };
-                    auto value_item = [&](int j) { return item + min(2 * j + 2, 2 * nj - 1); };
                     auto score_step = [&](int t, int j) {
                         if (j >= (t ? nt1 : nt0)) return;
                         if (j == 0) wait(&q_full[t], t ? nq1++ : nq0++);
-                        scores(t, key_item(j));
+                        scores(t, item + j);
                     };
                     auto value_step = [&](int t, int j) {
                         if (j >= (t ? nt1 : nt0)) return;
                         if (!wait(&p_full[t], t ? np1++ : np0++)) return;
                         tc_fence_after();
-                        values(t, value_item(j), j % FOLD != 0);
+                        values(t, item + j, j % FOLD != 0);
                     };
                     // the stages of a key (value) tile, once both query tiles' products with it are issued
                     auto keys_done = [&](int j) {
-                        tc_commit(&empty[key_item(j) % NS]);
+                        tc_commit(&k_empty[(item + j) % NK]);
                         if (j + 1 == nj) tc_commit(q_empty);
                     };
                     if constexpr (C::ALIAS) {
                         // a tile's next scores overwrite its probabilities, so they follow its value product
-                        ready(key_item(0));
+                        keys_ready(item);
                         score_step(0, 0);
                         score_step(1, 0);
                         keys_done(0);
                         for (int j = 0; j < nj && !*s_abort; ++j) {
                             const bool more = j + 1 < nj;
-                            if (more) ready(key_item(j + 1));
-                            ready(value_item(j));
+                            if (more) keys_ready(item + j + 1);
+                            values_ready(item + j);
                             value_step(0, j);
                             score_step(0, j + 1);
                             value_step(1, j);
                             score_step(1, j + 1);
-                            tc_commit(&empty[value_item(j) % NS]);
+                            tc_commit(&v_empty[(item + j) % NV]);
                             if (more) keys_done(j + 1);
                         }
-                    } else if (warp == C::SOFT + 1) {
+                    } else if (warp == 10) {
                         // scores go out as soon as their buffer was read
                         for (int j = 0; j < nj && !*s_abort; ++j) {
-                            ready(key_item(j));
+                            keys_ready(item + j);
                             score_step(0, j);
                             score_step(1, j);
                             keys_done(j);
@@ -947,18 +958,18 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     } else {
                         // value products as soon as the probabilities are there
                         for (int j = 0; j < nj && !*s_abort; ++j) {
-                            ready(value_item(j));
+                            values_ready(item + j);
                             value_step(0, j);
                             value_step(1, j);
-                            tc_commit(&empty[value_item(j) % NS]);
+                            tc_commit(&v_empty[(item + j) % NV]);
                         }
                     }
-                    item += 2 * nj;
+                    item += nj;
                 }
             }
         } else if (warp >= C::HELPER0) {
             const int ht = tid - 32 * C::HELPER0;  // thread among the helpers
-            uint32_t item = 0, cleaned = 0;  // cleaned: value tiles taken
+            uint32_t item = 0, cleaned = 0;        // tiles, value tiles cleaned
             for (int e = 0; !stop(); ++e) {
                 wait(&r_full[e % CU_RING], e / CU_RING);
                 RingUnit& R = ring(e);
@@ -968,14 +979,18 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 if constexpr (SRC == SRC_I8) {
                     // -------------------------------------------------- int8 tiles to fp16, as TMA would lay them out
                     constexpr int CH = D / 16;  // 16-value pieces of a row
-                    for (int k = 0; k < 2 * nj && !stop(); ++k, ++item) {
-                        const uint32_t rs = item % C::NR, st = item % NS;
-                        wait(&raw_full[rs], item / C::NR);
-                        if (item >= NS) wait(&empty[st], item / NS - 1);
-                        const uint4* src = reinterpret_cast<const uint4*>(smem + C::RAW_OFF + rs * C::RAW);
-                        uint8_t* dst = smem + C::KV_OFF + st * C::ITEM;
+                    // (two warps the keys, two the values)
+                    const bool is_v = ht >= 64;
+                    const int N = is_v ? NV : NK, hh = ht & 63;
+                    for (int j = 0; j < nj && !stop(); ++j, ++item) {
+                        constexpr uint32_t RR = RAWS > 0 ? RAWS : 1;
+                        const uint32_t rs = item % RR, st = item % N;
+                        wait((is_v ? rv_full : rk_full) + rs, item / RR);
+                        if (item >= N) wait((is_v ? v_empty : k_empty) + st, item / N - 1);
+                        const uint4* src = reinterpret_cast<const uint4*>(smem + C::RAW_OFF + ((is_v ? RAWS : 0) + rs) * C::RAW);
+                        uint8_t* dst = smem + C::KV_OFF + ((is_v ? NK : 0) + st) * C::ITEM;
 #pragma unroll 4
-                        for (int i = ht; i < CU_ROWS * CH; i += 32 * C::HELPERS) {
+                        for (int i = hh; i < CU_ROWS * CH; i += 64) {
                             const uint4 x = src[i];
                             const int row = i / CH, c = i % CH;
                             const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
@@ -994,22 +1009,20 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                         fence_proxy_async_smem();
                         __syncwarp();
                         if (lane == 0) {
-                            mbar_arrive(&raw_empty[rs]);
-                            mbar_arrive(&full[st]);
+                            mbar_arrive((is_v ? rv_empty : rk_empty) + rs);
+                            mbar_arrive((is_v ? v_full : k_full) + st);
                         }
                     }
                 } else {
                     // -------------------------------------------------- values that some row of the unit does not see
-                    // (the two warps take them in turn)
                     for (int j = max(0, dirty); j < nj && !stop(); ++j, ++cleaned) {
-                        if (int(cleaned % C::HELPERS) != ht >> 5) continue;
-                        const uint32_t it = item + min(2 * j + 2, 2 * nj - 1);
+                        const uint32_t st = (item + j) % NV;
                         wait(&dirty_full[cleaned % CU_CLEAN], cleaned / CU_CLEAN);
-                        uint8_t* v = smem + C::KV_OFF + (it % NS) * C::ITEM;
+                        uint8_t* v = smem + C::KV_OFF + (NK + st) * C::ITEM;
                         const int live_rows = keys - (kt0 + j) * CU_ROWS;  // rows from here on no token sees
                         bool odd = false;
 #pragma unroll 8
-                        for (int i = lane; i < C::ITEM / 16; i += 32) {
+                        for (int i = ht; i < C::ITEM / 16; i += 32 * C::HELPERS) {
                             uint4* at = reinterpret_cast<uint4*>(v + 16 * i);
                             uint4 x = *at;
                             const __half2 zero = __half2half2(__ushort_as_half(0));
@@ -1030,9 +1043,16 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                         if (odd) reinterpret_cast<volatile RingUnit&>(R).odd = 1;
                         fence_proxy_async_smem();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&full[it % NS]);
+                        // the last of the four warps hands the tile over
+                        if (lane == 0) {
+                            __threadfence_block();
+                            if (atomicAdd(s_clean + cleaned % CU_CLEAN, 1u) % C::HELPERS == C::HELPERS - 1) {
+                                __threadfence_block();
+                                mbar_arrive(&v_full[st]);
+                            }
+                        }
                     }
-                    item += 2 * nj;
+                    item += nj;
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&r_empty[e % CU_RING]);
@@ -1048,7 +1068,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == C::SOFT + 1) tc_dealloc(tmem, 512);
+    if (warp == 10) tc_dealloc(tmem, 512);
     if (tid == 0 && *s_abort) raise_error(p.error_flag, KVB_DEVERR_TIMEOUT);
 }
 
