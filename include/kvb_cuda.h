@@ -416,7 +416,8 @@ int kvb_paged_append(const kvb_append_args* args, void* stream);
  * total of -1 from the plan, too), or that has rows outside [0, num_tokens), gets NaN rows and sets bit
  * 1; a live block id outside the pool NaN rows and bit 2. error_word is required: zero it once, read
  * it when convenient. The workspace needs no preparation and holds nothing between calls. At most 64
- * query heads per KV head. q 16-byte aligned with a stride of whole 16 bytes, out 16-byte aligned. */
+ * query heads per KV head. q and the pools 16-byte aligned, q's stride whole 16 bytes; out and the
+ * workspace 32-byte aligned. */
 typedef struct kvb_chunk_args {
     kvb_shape shape;
     int q_type;               /* KVB_F32 or KVB_F16: q and out */

@@ -192,6 +192,14 @@ __device__ __forceinline__ void exp2_poly2(uint64_t x, float& a, float& b) {
     unpack2(y, a, b);
 }
 
+// 32 bytes in one store: each thread writes a row of its own, and its rows lie lines apart, so the number of
+// store instructions is what the outputs cost.
+__device__ __forceinline__ void store32(void* dst, const uint32_t* r) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
 // Pins the loaded values behind the wait that makes them valid.
 template <int N>
 __device__ __forceinline__ void pin(uint32_t* r) {
@@ -505,8 +513,13 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 if (masked) {
                     const int lim = limit - k0;
 #pragma unroll
-                    for (int c = 0; c < CU_ROWS; ++c)
-                        if (c >= lim) s[c] = 0xff800000u;  // -inf
+                    for (int c0 = 0; c0 < CU_ROWS; c0 += 32) {
+                        // one bit a key, so that a few instructions make the predicates
+                        const uint32_t sees = lim - c0 >= 32 ? ~0u : lim - c0 <= 0 ? 0u : (1u << (lim - c0)) - 1u;
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            if (!(sees >> c & 1u)) s[c0 + c] = 0xff800000u;  // -inf
+                    }
                 }
                 settled();  // the product that reads the probabilities before these
                 // The probabilities to tensor memory (QF32: hi, then lo halves of 32 keys, 16 columns each);
@@ -552,28 +565,33 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     return a + b;
                 };
                 // With the reference so far first. No probability is above their sum, so a sum in bounds needs
-                // no maximum. Otherwise (NaN included) the reference rises to the highest score, O and l
-                // follow, and the probabilities are computed again.
-                float sum = 0.f;
-                if (j > 0) sum = probabilities();
-                if (j == 0 || __any_sync(0xffffffffu, !(sum <= CU_MOST))) {
-                    float m0 = -INFINITY, m1 = -INFINITY;
+                // no maximum. Otherwise (NaN included, and at the first key tile) the reference rises to the
+                // highest score, O and l follow, and the probabilities are computed with that. (One copy of
+                // their code: the SM's instruction cache holds little more than the loop.)
+                float sum = 0.f, top = 0.f;
+                bool raise = j == 0;
+                for (;;) {
+                    if (raise) {
+                        float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < CU_ROWS; i += 4) {
-                        m0 = max3_nan(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                        m1 = max3_nan(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+                        for (int i = 0; i < CU_ROWS; i += 4) {
+                            m0 = max3_nan(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                            m1 = max3_nan(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+                        }
+                        top = fmaxf_nan(m0, m1) * f - CU_SHIFT;
+                        float scale = 1.f;
+                        if (top > ref) {
+                            scale = ref == -INFINITY ? 0.f : ex2(ref - top);
+                            ref = top;
+                            l *= scale;
+                        }
+                        if (j > 0) rescale(scale);
                     }
-                    const float top = fmaxf_nan(m0, m1) * f - CU_SHIFT;
-                    float scale = 1.f;
-                    if (top > ref) {
-                        scale = ref == -INFINITY ? 0.f : ex2(ref - top);
-                        ref = top;
-                        l *= scale;
-                    }
-                    if (j > 0) rescale(scale);
                     sum = probabilities();
-                    if (!(top < INFINITY)) sum = __int_as_float(0x7fc00000);  // a NaN or +inf score: the row is NaN
+                    if (raise || !__any_sync(0xffffffffu, !(sum <= CU_MOST))) break;
+                    raise = true;
                 }
+                if (!(top < INFINITY)) sum = __int_as_float(0x7fc00000);  // a NaN or +inf score: the row is NaN
                 l += sum;
                 tc_wait_st();
                 tc_fence_before();
@@ -631,14 +649,15 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     uint4* out = reinterpret_cast<uint4*>(slot >= 0 ? p.part_o + at * D + c
                                                                        : static_cast<float*>(p.out) + row * D + c);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) out[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    for (int i = 0; i < 4; ++i) store32(out + 2 * i, o + 8 * i);
                 } else {
                     uint4* out = reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + row * D + c);
-                    auto h2 = [&](int i) {
-                        return h2_as_u32(__floats2half2_rn(__uint_as_float(o[i]), __uint_as_float(o[i + 1])));
-                    };
+                    uint32_t h[16];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) out[i] = make_uint4(h2(8 * i), h2(8 * i + 2), h2(8 * i + 4), h2(8 * i + 6));
+                    for (int i = 0; i < 16; ++i)
+                        h[i] = h2_as_u32(__floats2half2_rn(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1])));
+                    store32(out, h);
+                    store32(out + 2, h + 8);
                 }
             }
             tc_fence_before();

@@ -15,6 +15,8 @@ int invalid(const char* msg) { return kvb_fail(KVB_ERR_INVALID, msg); }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
+
 int elem_size(int t) { return t == KVB_F32 ? 4 : t == KVB_F16 ? 2 : 1; }
 
 int launched(cudaError_t e) { return e == cudaSuccess ? KVB_OK : kvb_fail(KVB_ERR_DEVICE, cudaGetErrorString(e)); }
@@ -139,8 +141,8 @@ int run(Attend& a, void* workspace, size_t workspace_bytes, void* stream) {
     ChunkParams& p = a.p;
     if (a.s.batch == 0 || p.T == 0) return KVB_OK;
     if (int rc = geometry(a)) return rc;
-    if (!workspace || !aligned16(workspace) || workspace_bytes < (size_t)a.workspace)
-        return invalid("workspace null, not 16-byte aligned or too small");
+    if (!workspace || !aligned32(workspace) || workspace_bytes < (size_t)a.workspace)
+        return invalid("workspace null, not 32-byte aligned or too small");
     int sms = 0;
     if (int rc = kvb_device_sms(&sms)) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -198,8 +200,8 @@ int chunk_attend(const kvb_chunk_args* c, Attend& a) {
     if (!c->k || !c->v || !c->block_table || !c->total_lens || !c->cu_new || !c->out || !c->error_word)
         return invalid("null device pointer");
     if (c->kv_type == KVB_I8 && (!c->k_scale || !c->v_scale)) return invalid("i8 cache without scales");
-    if (!aligned16(c->out) || !aligned16(c->k) || !aligned16(c->v))
-        return invalid("out, k and v must be 16-byte aligned");
+    if (!aligned32(c->out) || !aligned16(c->k) || !aligned16(c->v))
+        return invalid("out must be 32-byte, k and v 16-byte aligned");
     if (c->num_blocks <= 0) return invalid("num_blocks must be > 0");
     return KVB_OK;
 }
@@ -233,7 +235,7 @@ int prompt_attend(const kvb_prompt_args* c, Attend& a) {
     if (int rc = check_rows(c->k, c->k_stride, kv_row, es, c->num_tokens)) return rc;
     if (int rc = check_rows(c->v, c->v_stride, kv_row, es, c->num_tokens)) return rc;
     if (!c->cu_lens || !c->out || !c->error_word) return invalid("null device pointer");
-    if (!aligned16(c->out)) return invalid("out must be 16-byte aligned");
+    if (!aligned32(c->out)) return invalid("out must be 32-byte aligned");
     return KVB_OK;
 }
 

@@ -85,7 +85,7 @@ def chunk_args(shape=kvb.Shape(2, 8, 2, 128), q=K.f16, kv=K.f16, page=16, max_bl
     (chunk_args(max_len=-1), "max_len"), (chunk_args(tokens=-1), "num_tokens"), (chunk_args(num_blocks=0), "num_blocks"),
     (chunk_args(kv=K.i8, v_scale=0), "scales"), (chunk_args(error_word=0), "null"), (chunk_args(out=0), "null"),
     (chunk_args(qp=0), "null"), (chunk_args(qp=0x1008), "16-byte"), (chunk_args(q_stride=1000), "stride"),
-    (chunk_args(q_stride=1028), "stride"), (chunk_args(out=0x7004), "16-byte"), (chunk_args(k=0x2008), "16-byte"),
+    (chunk_args(q_stride=1028), "stride"), (chunk_args(out=0x7004), "32-byte"), (chunk_args(out=0x7010), "32-byte"), (chunk_args(k=0x2008), "16-byte"),
     (chunk_args(kernel=kvb.Kernel.mma), "kernel"),
 ])
 def test_chunk_refusals(a, msg):
@@ -105,7 +105,7 @@ def prompt_args(shape=kvb.Shape(2, 8, 2, 64), type=K.f16, tokens=6, max_len=4, k
 @pytest.mark.parametrize("a,msg", [
     (prompt_args(type=K.i8), "f32 or f16"), (prompt_args(max_len=0), "max_new"), (prompt_args(q_stride=511), "stride"),
     (prompt_args(k_stride=127), "stride"), (prompt_args(v_stride=132), "stride"), (prompt_args(k=0x2004), "16-byte"),
-    (prompt_args(cu_lens=0), "null"), (prompt_args(v=0), "null"), (prompt_args(shape=kvb.Shape(2, 8, 2, 80)), "head_dim"),
+    (prompt_args(out=0x5010), "32-byte"), (prompt_args(cu_lens=0), "null"), (prompt_args(v=0), "null"), (prompt_args(shape=kvb.Shape(2, 8, 2, 80)), "head_dim"),
 ])
 def test_prompt_refusals(a, msg):
     with pytest.raises(ValueError, match=msg):
