@@ -290,7 +290,8 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
     __syncthreads();
     if (warp == 0) {  // exclusive sums, and the total behind them
         long long carry = 0;
-        for (int i = lane; i < C::THREADS; i += 32) {
+        const int used = (p.B + per - 1) / max(per, 1);  // threads that hold sequences
+        for (int i = lane; i < (used + 31) / 32 * 32; i += 32) {
             const long long v = s_sum[i];
             long long x = v;
 #pragma unroll
@@ -490,108 +491,196 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                         }
                     }
                 };
-                // the scores move to registers at once; with a buffer of their own it is free for the next ones
-                uint32_t s[CU_ROWS];
+                float sum = 0.f;
+                if constexpr (C::ALIAS) {
+                    // 32 keys at a time: hi, then lo halves, 16 columns each, over the scores they came from. The
+                    // reference is a whole number here, so that probabilities already written can follow it
+                    // exactly.
+                    settle_outputs();
+                    settled();
+#pragma unroll 1
+                    for (int c0 = 0; c0 < CU_ROWS; c0 += 32) {
+                        uint32_t s[32], pr[32];
+                        tc_ld32(ts + c0, s);
+                        tc_wait_ld();
+                        pin<32>(s);
+                        if constexpr (SRC == SRC_I8) {
 #pragma unroll
-                for (int c0 = 0; c0 < CU_ROWS; c0 += 32) tc_ld32(ts + c0, s + c0);
-                tc_wait_ld();
-                pin<CU_ROWS>(s);
-                if constexpr (!C::ALIAS) {
+                            for (int c = 0; c < 32; c += 8) {
+                                const float ks = scales[(c0 + c) >> lp];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) s[c + i] = __float_as_uint(__uint_as_float(s[c + i]) * ks);
+                            }
+                        }
+                        const int lim = limit - k0 - c0;
+                        if (masked) {
+                            const uint32_t sees = lim >= 32 ? ~0u : lim <= 0 ? 0u : (1u << lim) - 1u;
+#pragma unroll
+                            for (int c = 0; c < 32; ++c)
+                                if (!(sees >> c & 1u)) s[c] = 0xff800000u;  // -inf
+                        }
+                        float part = 0.f, top = 0.f;
+                        bool raise = j == 0 && c0 == 0;
+                        for (;;) {
+                            if (raise) {
+                                float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+                                for (int i = 0; i < 32; i += 4) {
+                                    m0 = max3_nan(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                                    m1 = max3_nan(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+                                }
+                                top = fmaxf_nan(m0, m1) * f;
+                                const float up = ceilf(top) - CU_SHIFT;
+                                float scale = 1.f;
+                                if (up > ref) {
+                                    scale = ref == -INFINITY ? 0.f : ex2(ref - up);
+                                    ref = up;
+                                    l *= scale;
+                                    sum *= scale;
+                                }
+                                if (j > 0) rescale(scale);
+                                const __half2 by = __float2half2_rn(scale);  // a power of two, or 0 when none is left
+#pragma unroll 1
+                                for (int c = 0; c < c0; c += 16) {
+                                    uint32_t w[16];
+                                    tc_ld16(tp + c, w);
+                                    tc_wait_ld();
+                                    pin<16>(w);
+#pragma unroll
+                                    for (int i = 0; i < 16; ++i) w[i] = h2_as_u32(__hmul2(u32_as_h2(w[i]), by));
+                                    tc_st16(tp + c, w);
+                                }
+                            }
+                            const float base = ref == -INFINITY ? 0.f : -ref;
+                            const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
+                            uint64_t l0 = 0, l1 = 0;
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) {
+                                float a, b;
+                                unpack2(fma2(pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, b2), a, b);
+                                a = ex2(a);
+                                b = ex2(b);
+                                if (i & 2) l1 = add2(l1, pack2(a, b));
+                                else l0 = add2(l0, pack2(a, b));
+                                if constexpr (SRC == SRC_I8) {
+                                    const float vs = scales[16 + ((c0 + i) >> lp)] * vexp;
+                                    a *= vs;
+                                    b *= vs;
+                                    if (masked) {  // the scale of a page that this row does not see may be anything
+                                        if (i >= lim) a = 0.f;
+                                        if (i + 1 >= lim) b = 0.f;
+                                    }
+                                }
+                                split_hi_lo(a, b, pr[i / 2], pr[16 + i / 2]);
+                            }
+                            float a, b;
+                            unpack2(add2(l0, l1), a, b);
+                            part = a + b;
+                            if (raise || !__any_sync(0xffffffffu, !(part <= CU_MOST))) break;
+                            raise = true;
+                        }
+                        tc_st32(tp + c0, pr);
+                        sum += top < INFINITY ? part : __int_as_float(0x7fc00000);
+                    }
+                } else {
+                    // the scores move to registers at once, and their buffer is free for the next ones
+                    uint32_t s[CU_ROWS];
+    #pragma unroll
+                    for (int c0 = 0; c0 < CU_ROWS; c0 += 32) tc_ld32(ts + c0, s + c0);
+                    tc_wait_ld();
+                    pin<CU_ROWS>(s);
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&s_free[t % C::SBUFS]);
-                }
-                settle_outputs();
-                if constexpr (SRC == SRC_I8) {
-#pragma unroll
-                    for (int c = 0; c < CU_ROWS; c += 8) {
-                        const float ks = scales[c >> lp];  // (pages of 128 tokens or more: one)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) s[c + i] = __float_as_uint(__uint_as_float(s[c + i]) * ks);
+                    settle_outputs();
+                    if constexpr (SRC == SRC_I8) {
+    #pragma unroll
+                        for (int c = 0; c < CU_ROWS; c += 8) {
+                            const float ks = scales[c >> lp];  // (pages of 128 tokens or more: one)
+    #pragma unroll
+                            for (int i = 0; i < 8; ++i) s[c + i] = __float_as_uint(__uint_as_float(s[c + i]) * ks);
+                        }
                     }
-                }
-                if (masked) {
-                    const int lim = limit - k0;
-#pragma unroll
-                    for (int c0 = 0; c0 < CU_ROWS; c0 += 32) {
-                        // one bit a key, so that a few instructions make the predicates
-                        const uint32_t sees = lim - c0 >= 32 ? ~0u : lim - c0 <= 0 ? 0u : (1u << (lim - c0)) - 1u;
-#pragma unroll
-                        for (int c = 0; c < 32; ++c)
-                            if (!(sees >> c & 1u)) s[c0 + c] = 0xff800000u;  // -inf
+                    if (masked) {
+                        const int lim = limit - k0;
+    #pragma unroll
+                        for (int c0 = 0; c0 < CU_ROWS; c0 += 32) {
+                            // one bit a key, so that a few instructions make the predicates
+                            const uint32_t sees = lim - c0 >= 32 ? ~0u : lim - c0 <= 0 ? 0u : (1u << (lim - c0)) - 1u;
+    #pragma unroll
+                            for (int c = 0; c < 32; ++c)
+                                if (!(sees >> c & 1u)) s[c0 + c] = 0xff800000u;  // -inf
+                        }
                     }
-                }
-                settled();  // the product that reads the probabilities before these
-                // The probabilities to tensor memory (QF32: hi, then lo halves of 32 keys, 16 columns each);
-                // their sum.
-                auto probabilities = [&]() {
-                    const float base = ref == -INFINITY ? 0.f : -ref;
-                    const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
-                    uint64_t l0 = 0, l1 = 0;
-#pragma unroll
-                    for (int c0 = 0; c0 < CU_ROWS; c0 += 32) {
-                        uint32_t pr[QF32 ? 32 : 16];
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const uint64_t x =
-                                fma2(pack2(__uint_as_float(s[c0 + i]), __uint_as_float(s[c0 + i + 1])), f2, b2);
-                            float a, b;
-                            if (!QF32 && (i / 2) % CU_POLY_OF < CU_POLY) {
-                                exp2_poly2(x, a, b);
-                            } else {
-                                unpack2(x, a, b);
-                                a = ex2(a);
-                                b = ex2(b);
-                            }
-                            if (i & 2) l1 = add2(l1, pack2(a, b));
-                            else l0 = add2(l0, pack2(a, b));
-                            if constexpr (SRC == SRC_I8) {
-                                const float vs = scales[16 + ((c0 + i) >> lp)] * vexp;
-                                a *= vs;
-                                b *= vs;
-                                if (masked) {  // the scale of a page that this row does not see may be anything
-                                    if (k0 + c0 + i >= limit) a = 0.f;
-                                    if (k0 + c0 + i + 1 >= limit) b = 0.f;
+                    settled();  // the product that reads the probabilities before these
+                    // The probabilities to tensor memory; their sum.
+                    auto probabilities = [&]() {
+                        const float base = ref == -INFINITY ? 0.f : -ref;
+                        const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
+                        uint64_t l0 = 0, l1 = 0;
+    #pragma unroll
+                        for (int c0 = 0; c0 < CU_ROWS; c0 += 32) {
+                            uint32_t pr[16];
+    #pragma unroll
+                            for (int i = 0; i < 32; i += 2) {
+                                const uint64_t x =
+                                    fma2(pack2(__uint_as_float(s[c0 + i]), __uint_as_float(s[c0 + i + 1])), f2, b2);
+                                float a, b;
+                                if ((i / 2) % CU_POLY_OF < CU_POLY) {
+                                    exp2_poly2(x, a, b);
+                                } else {
+                                    unpack2(x, a, b);
+                                    a = ex2(a);
+                                    b = ex2(b);
                                 }
+                                if (i & 2) l1 = add2(l1, pack2(a, b));
+                                else l0 = add2(l0, pack2(a, b));
+                                if constexpr (SRC == SRC_I8) {
+                                    const float vs = scales[16 + ((c0 + i) >> lp)] * vexp;
+                                    a *= vs;
+                                    b *= vs;
+                                    if (masked) {  // the scale of a page that this row does not see may be anything
+                                        if (k0 + c0 + i >= limit) a = 0.f;
+                                        if (k0 + c0 + i + 1 >= limit) b = 0.f;
+                                    }
+                                }
+                                pr[i / 2] = h2_as_u32(__floats2half2_rn(a, b));
                             }
-                            if constexpr (QF32) split_hi_lo(a, b, pr[i / 2], pr[16 + i / 2]);
-                            else pr[i / 2] = h2_as_u32(__floats2half2_rn(a, b));
+                            tc_st16(tp + c0 / 2, pr);
                         }
-                        if constexpr (QF32) tc_st32(tp + c0, pr);
-                        else tc_st16(tp + c0 / 2, pr);
+                        float a, b;
+                        unpack2(add2(l0, l1), a, b);
+                        return a + b;
+                    };
+                    // With the reference so far first. No probability is above their sum, so a sum in bounds needs
+                    // no maximum. Otherwise (NaN included, and at the first key tile) the reference rises to the
+                    // highest score, O and l follow, and the probabilities are computed with that. (One copy of
+                    // their code: the SM's instruction cache holds little more than the loop.)
+                    float top = 0.f;
+                    bool raise = j == 0;
+                    for (;;) {
+                        if (raise) {
+                            float m0 = -INFINITY, m1 = -INFINITY;
+    #pragma unroll
+                            for (int i = 0; i < CU_ROWS; i += 4) {
+                                m0 = max3_nan(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                                m1 = max3_nan(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+                            }
+                            top = fmaxf_nan(m0, m1) * f - CU_SHIFT;
+                            float scale = 1.f;
+                            if (top > ref) {
+                                scale = ref == -INFINITY ? 0.f : ex2(ref - top);
+                                ref = top;
+                                l *= scale;
+                            }
+                            if (j > 0) rescale(scale);
+                        }
+                        sum = probabilities();
+                        if (raise || !__any_sync(0xffffffffu, !(sum <= CU_MOST))) break;
+                        raise = true;
                     }
-                    float a, b;
-                    unpack2(add2(l0, l1), a, b);
-                    return a + b;
-                };
-                // With the reference so far first. No probability is above their sum, so a sum in bounds needs
-                // no maximum. Otherwise (NaN included, and at the first key tile) the reference rises to the
-                // highest score, O and l follow, and the probabilities are computed with that. (One copy of
-                // their code: the SM's instruction cache holds little more than the loop.)
-                float sum = 0.f, top = 0.f;
-                bool raise = j == 0;
-                for (;;) {
-                    if (raise) {
-                        float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-                        for (int i = 0; i < CU_ROWS; i += 4) {
-                            m0 = max3_nan(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                            m1 = max3_nan(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
-                        }
-                        top = fmaxf_nan(m0, m1) * f - CU_SHIFT;
-                        float scale = 1.f;
-                        if (top > ref) {
-                            scale = ref == -INFINITY ? 0.f : ex2(ref - top);
-                            ref = top;
-                            l *= scale;
-                        }
-                        if (j > 0) rescale(scale);
-                    }
-                    sum = probabilities();
-                    if (raise || !__any_sync(0xffffffffu, !(sum <= CU_MOST))) break;
-                    raise = true;
+                    if (!(top < INFINITY)) sum = __int_as_float(0x7fc00000);  // a NaN or +inf score: the row is NaN
                 }
-                if (!(top < INFINITY)) sum = __int_as_float(0x7fc00000);  // a NaN or +inf score: the row is NaN
                 l += sum;
                 tc_wait_st();
                 tc_fence_before();

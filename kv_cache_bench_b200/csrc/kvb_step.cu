@@ -18,7 +18,7 @@
 
 #include <algorithm>
 
-#include "kvb_device.cuh"
+#include "kvb_quant.cuh"
 #include "kvb_step.h"
 
 namespace {
@@ -187,8 +187,8 @@ __global__ void __launch_bounds__(AP_THREADS) append_rows_kernel(const AppendPar
             const long long i = i0 + u * step;
             dst[u] = -1;
             if (i >= total) continue;
-            // a token's pieces are below 2^31 (checked by the host)
-            const long long t = i / per_token;
+            // a token's pieces are below 2^31 (checked by the host), mostly all of them are
+            const long long t = total < (1ll << 31) ? kvb_div(int(i), p.div_token) : i / per_token;
             const int in = int(i - t * per_token), h = kvb_div(in, p.div_row), c = in - h * int(p.div_row.d);
             const long long slot = __ldg(p.slot_map + t);
             if (slot < 0 || slot >= limit) {
@@ -240,37 +240,32 @@ __device__ __forceinline__ float amax4(float4 v) {
     return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
 }
 
-// clamp(rint(x / scale)), the page quantizer's rule (kvb_pages.cu), four values packed low byte first.
-__device__ __forceinline__ uint32_t quantize4(const float4 v, float scale) {
-    const float x[4] = {v.x, v.y, v.z, v.w};
-    uint32_t packed = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int q = min(max(__float2int_rn(__fdiv_rn(x[e], scale)), -127), 127);
-        packed |= uint32_t(q & 255) << (8 * e);
-    }
-    return packed;
-}
+// int8 pools. A run is the new tokens of one sequence that share a page, for one KV head of K or V, and TPR
+// threads (a warp, or the CTA for pages of 32 KB of fp32 and more) take it. The page's scale becomes
+// s = max(s_old, amax / 127) (s_old only if the page had rows before); rows that were there are rounded
+// again, rint(q * (s_old / s)), when the scale grew; new rows by the page quantizer's rule (kvb_quant.cuh). A
+// token starts a run if it is its sequence's first new one or the first of its page; each group looks for
+// them among `tpg` tokens. A run of up to AP_REGS float4 per thread stays in registers between the maximum
+// and the rounding, a larger one is read again (from L1 or L2). Bound by memory; with a warp for every run
+// and two reads, prompts of 7 k tokens into pages of 128 took 120 us.
+constexpr int AP_REGS = 16;
 
-// int8 pools. A run is the new tokens of one sequence that share a page, for one KV head of K or V: one
-// warp each. The page's scale becomes s = max(s_old, amax / 127) (s_old only if the page had rows
-// before); rows that were there are rounded again, rint(q * (s_old / s)), when the scale grew. Warps
-// look for runs among `tpw` tokens at a time: a token starts a run if it is its sequence's first new
-// one or the first of its page.
-template <typename SRC>
-__global__ void __launch_bounds__(AP_THREADS) append_i8_kernel(const AppendParams p, int tpw) {
-    const int lane = threadIdx.x & 31;
-    const int h = blockIdx.y >> 1, which = blockIdx.y & 1;
-    const long long wid = (long long)blockIdx.x * (AP_THREADS / 32) + (threadIdx.x >> 5);
-    const long long tok0 = wid * tpw;
+template <typename SRC, int TPR>
+__global__ void __launch_bounds__(AP_THREADS) append_i8_kernel(const AppendParams p, int tpg) {
+    constexpr int WARPS = TPR / 32;
+    __shared__ int s_tok[AP_THREADS], s_n[AP_THREADS], s_at[AP_THREADS];  // a CTA-wide group's runs
+    __shared__ long long s_block[AP_THREADS];
+    __shared__ int s_runs;
+    __shared__ float s_max[2][AP_THREADS / 32];
+    const int lane = threadIdx.x & 31, gl = threadIdx.x % TPR;
+    const long long tok0 = ((long long)blockIdx.x * (AP_THREADS / TPR) + threadIdx.x / TPR) * tpg;
     pdl_wait();
     pdl_trigger();
-    if (tok0 >= p.num_tokens) return;
-    // each of the first tpw lanes decodes one token
-    const int t = int(tok0) + lane;
+    // each of the first tpg threads of a group decodes one token
+    const int t = int(min(tok0 + gl, (long long)p.num_tokens));
     int n = 0, at = 0;
     long long block = -1;
-    if (lane < tpw && t < p.num_tokens) {
+    if (gl < tpg && t < p.num_tokens) {
         int lo = 0, hi = p.B;  // the first sequence that ends behind t
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
@@ -303,33 +298,43 @@ __global__ void __launch_bounds__(AP_THREADS) append_i8_kernel(const AppendParam
         }
     }
     const int dw = int(p.div_row.d);  // pieces of four values per row
-    const SRC* src = static_cast<const SRC*>(p.src[which]) + (long long)h * p.D;
-    const long long stride = p.stride[which];
-    for (unsigned runs = __ballot_sync(0xffffffffu, block >= 0); runs; runs &= runs - 1) {
-        const int l = __ffs(runs) - 1;
-        const int rn = __shfl_sync(0xffffffffu, n, l), rat = __shfl_sync(0xffffffffu, at, l);
-        const long long rb = __shfl_sync(0xffffffffu, block, l) * p.Hkv + h;
-        const SRC* rows = src + (tok0 + l) * stride;
+    int parity = 0;  // alternates the CTA-wide reduction's slots
+    auto run = [&](int y, int rt, int rn, int rat, long long rblock) {
+        const int h = y >> 1, which = y & 1;
+        const SRC* src = static_cast<const SRC*>(p.src[which]) + (long long)h * p.D;
+        const long long stride = p.stride[which];
+        const long long rb = rblock * p.Hkv + h;
+        const SRC* rows = src + rt * stride;
         uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<int8_t*>(p.pool[which]) + rb * p.page * p.D);
         const int pieces = rn * dw;  // below 2^31: a page of one head is (checked by the host)
+        const bool keep = pieces <= TPR * AP_REGS;
+        float4 v[AP_REGS];
         float amax = 0.f;
-        constexpr int U = 8;
-        for (int i0 = lane; i0 < pieces; i0 += 32 * U) {
-            float4 v[U];
+        auto load = [&](int i0) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = i0 + 32 * u;
+            for (int u = 0; u < AP_REGS; ++u) {
+                const int i = i0 + TPR * u;
                 v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (i < pieces) {
                     const int r = kvb_div(i, p.div_row);
                     v[u] = load4(rows + r * stride + 4 * (i - r * dw));
                 }
             }
+        };
+        for (int i0 = gl; i0 < pieces; i0 += TPR * AP_REGS) {
+            load(i0);
 #pragma unroll
-            for (int u = 0; u < U; ++u) amax = fmaxf(amax, amax4(v[u]));
+            for (int u = 0; u < AP_REGS; ++u) amax = fmaxf(amax, amax4(v[u]));
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if constexpr (WARPS > 1) {
+            if (lane == 0) s_max[parity][threadIdx.x >> 5] = amax;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < WARPS; ++i) amax = fmaxf(amax, s_max[parity][i]);
+            parity ^= 1;
+        }
         float scale = amax / 127.0f;
         if (rat > 0) {
             const float old = p.scale[which][rb];
@@ -337,7 +342,7 @@ __global__ void __launch_bounds__(AP_THREADS) append_i8_kernel(const AppendParam
                 scale = old;
             } else {
                 const float ratio = __fdiv_rn(old, scale);
-                for (int i = lane; i < rat * dw; i += 32) {
+                for (int i = gl; i < rat * dw; i += TPR) {
                     const uint32_t x = dst[i];
                     uint32_t y = 0;
 #pragma unroll
@@ -349,24 +354,45 @@ __global__ void __launch_bounds__(AP_THREADS) append_i8_kernel(const AppendParam
                 }
             }
         }
-        __syncwarp();  // every lane has read the old scale
-        if (lane == 0) p.scale[which][rb] = scale;
+        if constexpr (WARPS > 1) __syncthreads();  // every thread has read the old scale
+        else __syncwarp();
+        if (gl == 0) p.scale[which][rb] = scale;
         dst += rat * dw;
-        for (int i0 = lane; i0 < pieces; i0 += 32 * U) {
-            float4 v[U];
+        const float rcp = finite_rcp(scale);
+        for (int i0 = gl; i0 < pieces; i0 += TPR * AP_REGS) {
+            if (!keep) load(i0);
+            int near = scale > 0.f && rcp == 0.f;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = i0 + 32 * u;
-                if (i < pieces) {
-                    const int r = kvb_div(i, p.div_row);
-                    v[u] = load4(rows + r * stride + 4 * (i - r * dw));
+            for (int u = 0; u < AP_REGS; ++u) {
+                const int i = i0 + TPR * u;
+                if (i < pieces) dst[i] = scale > 0.f ? quantize4_fast(v[u], rcp, near) : 0u;
+            }
+            if (near) {
+#pragma unroll
+                for (int u = 0; u < AP_REGS; ++u) {
+                    const int i = i0 + TPR * u;
+                    if (i < pieces) dst[i] = quantize4_exact(v[u], scale);
                 }
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = i0 + 32 * u;
-                if (i < pieces) dst[i] = scale > 0.f ? quantize4(v[u], scale) : 0u;
-            }
+        }
+    };
+    if constexpr (WARPS > 1) {
+        if (threadIdx.x == 0) s_runs = 0;
+        __syncthreads();
+        if (block >= 0) {
+            const int i = atomicAdd(&s_runs, 1);  // (their order does not matter: a page has one run)
+            s_tok[i] = t, s_n[i] = n, s_at[i] = at, s_block[i] = block;
+        }
+        __syncthreads();
+        for (int y = blockIdx.y; y < 2 * p.Hkv; y += gridDim.y)
+            for (int i = 0; i < s_runs; ++i) run(y, s_tok[i], s_n[i], s_at[i], s_block[i]);
+    } else {
+        for (unsigned runs = __ballot_sync(0xffffffffu, block >= 0); runs; runs &= runs - 1) {
+            const int l = __ffs(runs) - 1;
+            const int rt = __shfl_sync(0xffffffffu, t, l), rn = __shfl_sync(0xffffffffu, n, l);
+            const int rat = __shfl_sync(0xffffffffu, at, l);
+            const long long rblock = __shfl_sync(0xffffffffu, block, l);
+            for (int y = blockIdx.y; y < 2 * p.Hkv; y += gridDim.y) run(y, rt, rn, rat, rblock);
         }
     }
 }
@@ -389,12 +415,20 @@ cudaError_t launch_rows(const AppendParams& p, int num_sms, cudaStream_t stream)
 
 template <typename SRC>
 cudaError_t launch_i8(const AppendParams& p, int num_sms, cudaStream_t stream) {
-    // tokens a warp looks at: one while that keeps the grid small, up to 32 (most are no run's first)
-    int tpw = 1;
-    while (tpw < 32 && (long long)p.num_tokens / tpw * p.Hkv * 2 > (long long)num_sms * 64) tpw *= 2;
-    const long long warps = ((long long)p.num_tokens + tpw - 1) / tpw;
+    // A CTA for every run where a page of one head is large and the step mean is more than a few rows a
+    // sequence; it looks at 128 tokens. Otherwise a warp, which looks at one token while that keeps the grid
+    // small, up to 32 (most are no run's first).
+    const bool cta = (long long)p.page * p.D * 4 >= 32768 && p.num_tokens >= 8ll * p.B;
+    int tpg = cta ? 128 : 1;
+    if (!cta)
+        while (tpg < 32 && (long long)p.num_tokens / tpg * p.Hkv * 2 > (long long)num_sms * 64) tpg *= 2;
+    const long long groups = ((long long)p.num_tokens + tpg - 1) / tpg, per = cta ? 1 : AP_THREADS / 32;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((warps + AP_THREADS / 32 - 1) / (AP_THREADS / 32)), 2 * p.Hkv);
+    // heads of K and V side by side, as many as make four CTAs an SM (the others follow in the same CTA, which
+    // knows its runs already)
+    const long long x = (groups + per - 1) / per;
+    const long long y = std::min<long long>(2ll * p.Hkv, std::max<long long>(1, (4ll * num_sms + x - 1) / x));
+    cfg.gridDim = dim3((unsigned)x, (unsigned)y);
     cfg.blockDim = dim3(AP_THREADS);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -402,7 +436,8 @@ cudaError_t launch_i8(const AppendParams& p, int num_sms, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, append_i8_kernel<SRC>, p, tpw);
+    return cta ? cudaLaunchKernelEx(&cfg, append_i8_kernel<SRC, AP_THREADS>, p, tpg)
+               : cudaLaunchKernelEx(&cfg, append_i8_kernel<SRC, 32>, p, tpg);
 }
 
 }  // namespace

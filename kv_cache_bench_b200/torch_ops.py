@@ -13,9 +13,10 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import Kernel, KvType, Shape, append_args, chunk_args, device_args, paged_append, paged_chunk_async, \
-    paged_chunk_workspace_bytes, paged_decode_async, paged_error_flag, paged_part_tokens, paged_workspace_bytes, \
-    prompt_args, prompt_async, prompt_workspace_bytes, step_plan, step_plan_args
+from . import Kernel, KvType, Shape, _CAppendArgs, _CChunkArgs, _CPromptArgs, _CShape, _CStepPlanArgs, device_args, \
+    paged_append, paged_chunk_async, paged_chunk_workspace_bytes, paged_decode_async, paged_error_flag, \
+    paged_part_tokens, paged_workspace_bytes, prompt_async, prompt_workspace_bytes, step_plan
+
 
 _KV_DTYPE = {KvType.f32: torch.float32, KvType.f16: torch.float16, KvType.i8: torch.int8}
 
@@ -84,40 +85,55 @@ class PagedDecoder:
 
 
 # ---- serving steps of several new tokens per sequence ------------------------------------------------
+# These calls sit on a decode step's critical path, a few microseconds of GPU work each: the checks below
+# are written for little host time.
 
 _NO_GUARD = contextlib.nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_INT32, _INT64, _F32, _I8 = torch.int32, torch.int64, torch.float32, torch.int8
+_KV_TYPE = {v: int(k) for k, v in _KV_DTYPE.items()}
 
 
-def _on(device: torch.device):
-    """Makes `device` current for a launch (nothing to do where it is already)."""
-    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _on(index: int):
+    """Makes device `index` current for a launch (nothing to do where it is already)."""
+    return _NO_GUARD if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def _type(name: str, t) -> int:
+    k = _KV_TYPE.get(t.dtype)
+    if k is None:
+        raise ValueError(f"unsupported {name} dtype {t.dtype}")
+    return k
 
 
-def _tensor(name: str, t, dtype, device, shape=None) -> int:
-    """The address of a contiguous tensor of this type, place and shape."""
-    if t.dtype is not dtype or t.device != device or not t.is_contiguous() or (shape is not None and t.shape != shape):
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor"
-                         f"{'' if shape is None else ' of shape ' + str(tuple(shape))} on {device}")
+def _tensor(name: str, t, dtype, index: int, shape) -> int:
+    """The address of a contiguous tensor of this type, device and shape."""
+    if t.dtype is not dtype or t.get_device() != index or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{index}")
     return t.data_ptr()
 
 
-def _rows(name: str, t, device) -> int:
+def _rows(name: str, t, index: int) -> int:
     """The token stride of [tokens][heads][dim] rows; a token's own values lie together."""
-    if t.dim() != 3 or t.device != device or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
-        raise ValueError(f"{name} must be [tokens][heads][dim] on {device}, with each token's heads contiguous")
-    return t.stride(0)
+    if t.dim() == 3 and t.get_device() == index:
+        a, b, c = t.stride()
+        if c == 1 and b == t.shape[2]:
+            return a
+    raise ValueError(f"{name} must be [tokens][heads][dim] on cuda:{index}, with each token's heads contiguous")
 
 
-def _error(error_word, device) -> int:
+def _error(error_word, index: int):
     if error_word is None:
-        return 0
-    if error_word.dtype not in (torch.int32, torch.uint32) or error_word.device != device or error_word.numel() < 1:
-        raise ValueError(f"error_word must be an int32 tensor on {device}")
+        return None
+    if error_word.dtype not in (torch.int32, torch.uint32) or error_word.get_device() != index or error_word.numel() < 1:
+        raise ValueError(f"error_word must be an int32 tensor on cuda:{index}")
     return error_word.data_ptr()
+
+
+def _table(block_table, batch: int, index: int):
+    if block_table.dim() != 2 or block_table.shape[0] != batch:
+        raise ValueError("block_table must be [batch][max_blocks]")
+    return _tensor("block_table", block_table, _INT32, index, block_table.shape), block_table.shape[1]
 
 
 class StepPlan(NamedTuple):
@@ -140,76 +156,74 @@ def plan_step(seq_lens, new_lens, block_table, ring, ring_pos, *, page_size: int
     ``ring_pos[1] += m``. `num_tokens` is the length of the packed step (the sum of `new_lens`, or more).
     `error_word`, an int32 tensor, collects the error bits.
     """
-    device = seq_lens.device
-    if device.type != "cuda":
+    index = seq_lens.get_device()
+    if index < 0:
         raise ValueError("plan_step takes CUDA tensors")
+    if num_tokens < 0 or seq_lens.dim() != 1 or ring.dim() != 1:
+        raise ValueError("num_tokens < 0, or seq_lens or ring not one-dimensional")
     batch = seq_lens.shape[0]
-    if block_table.dim() != 2 or block_table.shape[0] != batch:
-        raise ValueError("block_table must be [batch][max_blocks]")
-    if num_tokens < 0:
-        raise ValueError("num_tokens < 0")
-    new = lambda n, dtype: torch.empty(n, dtype=dtype, device=device)  # noqa: E731
-    p = StepPlan(new(batch, torch.int32), new(batch + 1, torch.int32), new(num_tokens, torch.int64),
-                 new(num_tokens, torch.int32), new(2, torch.int64))
-    a = step_plan_args(
-        batch, page_size, block_table.shape[1], num_tokens,
-        seq_lens=_tensor("seq_lens", seq_lens, torch.int32, device, (batch,)),
-        new_lens=_tensor("new_lens", new_lens, torch.int32, device, (batch,)),
-        block_table=_tensor("block_table", block_table, torch.int32, device),
-        ring=_tensor("ring", ring, torch.int32, device), ring_pos=_tensor("ring_pos", ring_pos, torch.int64, device, (2,)),
-        ring_out=p.ring_pos.data_ptr(), total_lens=p.total_lens.data_ptr(), cu_new=p.cu_new.data_ptr(),
-        slot_map=p.slot_map.data_ptr(), positions=p.positions.data_ptr(), ring_size=ring.numel(),
-        num_blocks=num_blocks, error_word=_error(error_word, device))
-    with _on(device):
-        step_plan(a, _stream(device))
+    lens = _tensor("seq_lens", seq_lens, _INT32, index, (batch,))
+    pos = _tensor("ring_pos", ring_pos, _INT64, index, (2,))
+    table, max_blocks = _table(block_table, batch, index)
+    p = StepPlan(torch.empty_like(seq_lens), seq_lens.new_empty(batch + 1), ring_pos.new_empty(num_tokens),
+                 seq_lens.new_empty(num_tokens), torch.empty_like(ring_pos))
+    a = _CStepPlanArgs(batch, page_size, max_blocks, num_tokens, lens,
+                       _tensor("new_lens", new_lens, _INT32, index, (batch,)), table,
+                       _tensor("ring", ring, _INT32, index, ring.shape), pos, p.ring_pos.data_ptr(),
+                       p.total_lens.data_ptr(), p.cu_new.data_ptr(), p.slot_map.data_ptr(), p.positions.data_ptr(),
+                       ring.shape[0], num_blocks, _error(error_word, index))
+    with _on(index):
+        step_plan(a, _raw_stream(index))
     return p
 
 
-def _append(k, v, k_pool, v_pool, error_word, batch=0, **kw):
-    device = k_pool.device
-    if device.type != "cuda":
-        raise ValueError("the pools must be CUDA tensors")
-    if k.shape != v.shape or k.dtype != v.dtype:
+def _append(k, v, k_pool, v_pool, index, slots, batch, max_blocks, scales, lists, error_word):
+    if k.shape != v.shape or k.dtype is not v.dtype:
         raise ValueError("k and v must have one shape and type")
-    k_stride, v_stride = _rows("k", k, device), _rows("v", v, device)
-    if k_pool.dim() != 4 or k_pool.shape[1] != k.shape[1] or k_pool.shape[3] != k.shape[2]:
+    k_stride, v_stride = _rows("k", k, index), _rows("v", v, index)
+    T, Hkv, D = k.shape
+    pool = k_pool.shape
+    if len(pool) != 4 or pool[1] != Hkv or pool[3] != D:
         raise ValueError("pools must be [num_blocks][kv_heads][page][dim], heads and dim those of k")
-    _tensor("v_pool", v_pool, k_pool.dtype, device, k_pool.shape)
-    _tensor("k_pool", k_pool, k_pool.dtype, device)
-    a = append_args(batch, k.shape[1], k.shape[2], kv_type_of(k), kv_type_of(k_pool), k_pool.shape[2], k.shape[0],
-                    k=k.data_ptr(), v=v.data_ptr(), k_stride=k_stride, v_stride=v_stride, k_pool=k_pool.data_ptr(),
-                    v_pool=v_pool.data_ptr(), num_blocks=k_pool.shape[0], error_word=_error(error_word, device), **kw)
-    with _on(device):
-        paged_append(a, _stream(device))
+    a = _CAppendArgs(_CShape(batch, Hkv, Hkv, D), _type("k", k), _type("pool", k_pool), pool[2], max_blocks, T,
+                     k.data_ptr(), v.data_ptr(), k_stride, v_stride,
+                     _tensor("k_pool", k_pool, k_pool.dtype, index, pool),
+                     _tensor("v_pool", v_pool, k_pool.dtype, index, pool), *scales, pool[0], slots, *lists,
+                     _error(error_word, index))
+    with _on(index):
+        paged_append(a, _raw_stream(index))
 
 
 def append_kv(k, v, k_pool, v_pool, *, slot_map, error_word=None) -> None:
     """New tokens' keys and values (fp32 or fp16 [tokens][kv_heads][dim], any token stride of whole 16
     bytes) into fp32 or fp16 pages, at the plan's `slot_map` (kvb_paged_append)."""
-    if k_pool.dtype == torch.int8:
+    if k_pool.dtype is _I8:
         raise ValueError("int8 pages are written by append_kv_i8")
-    _append(k, v, k_pool, v_pool, error_word,
-            slot_map=_tensor("slot_map", slot_map, torch.int64, k_pool.device, (k.shape[0],)))
+    index = k_pool.get_device()
+    if index < 0:
+        raise ValueError("the pools must be CUDA tensors")
+    slots = _tensor("slot_map", slot_map, _INT64, index, k.shape[:1])
+    _append(k, v, k_pool, v_pool, index, slots, 0, 0, (None, None), (None, None, None), error_word)
 
 
 def append_kv_i8(k, v, k_pool, v_pool, k_scale, v_scale, *, block_table, total_lens, cu_new, error_word=None) -> None:
     """New tokens' keys and values quantized into int8 pages; the scales ([num_blocks][kv_heads]) and
     the rows of pages that were begun follow where a larger value needs it (kvb_paged_append)."""
-    if k_pool.dtype != torch.int8:
+    if k_pool.dtype is not _I8:
         raise ValueError("append_kv_i8 writes int8 pages")
-    device, batch = k_pool.device, total_lens.shape[0]
-    if block_table.dim() != 2 or block_table.shape[0] != batch:
-        raise ValueError("block_table must be [batch][max_blocks]")
+    index, batch = k_pool.get_device(), total_lens.shape[0]
+    if index < 0:
+        raise ValueError("the pools must be CUDA tensors")
+    table, max_blocks = _table(block_table, batch, index)
     if batch == 0:
         if k.shape[0]:
             raise ValueError("tokens without a sequence")
         return
-    scale = lambda n, t: _tensor(n, t, torch.float32, device, k_pool.shape[:2])  # noqa: E731
-    _append(k, v, k_pool, v_pool, error_word, batch, k_scale=scale("k_scale", k_scale),
-            v_scale=scale("v_scale", v_scale), max_blocks=block_table.shape[1],
-            block_table=_tensor("block_table", block_table, torch.int32, device),
-            total_lens=_tensor("total_lens", total_lens, torch.int32, device, (batch,)),
-            cu_new=_tensor("cu_new", cu_new, torch.int32, device, (batch + 1,)))
+    scales = k_pool.shape[:2]
+    _append(k, v, k_pool, v_pool, index, None, batch, max_blocks,
+            (_tensor("k_scale", k_scale, _F32, index, scales), _tensor("v_scale", v_scale, _F32, index, scales)),
+            (table, _tensor("total_lens", total_lens, _INT32, index, (batch,)),
+             _tensor("cu_new", cu_new, _INT32, index, (batch + 1,))), error_word)
 
 
 class PagedPrefill:
@@ -225,61 +239,55 @@ class PagedPrefill:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self.error_word = torch.zeros(1, dtype=torch.int32, device=self.device)
 
-    def _out(self, q, out):
-        if out is None:
-            return torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        _tensor("out", out, q.dtype, self.device, q.shape)
-        return out
+    def _run(self, a, workspace_bytes, launch, index):
+        with _on(index):
+            n = workspace_bytes(a)
+            workspace = self.error_word.new_empty((n + 3) // 4)
+            launch(a, workspace.data_ptr(), n, _raw_stream(index))
 
     def chunk(self, q, k_pool, v_pool, block_table, total_lens, cu_new, *, max_new: int, max_len: int, k_scale=None,
               v_scale=None, out=None, kernel=Kernel.auto):
         """New token i of sequence b (packed row cu_new[b] + i) over the tokens at positions up to its own,
         total_lens[b] - n_b + i; the pages hold the new tokens already (kvb_paged_chunk_async)."""
-        device = self.device
-        q_stride = _rows("q", q, device)
+        index = self.device.index
+        q_stride = _rows("q", q, index)
         T, H, D = q.shape
-        if k_pool.dim() != 4 or k_pool.shape[3] != D:
+        pool = k_pool.shape
+        if len(pool) != 4 or pool[3] != D:
             raise ValueError("pools must be [num_blocks][kv_heads][page][dim], dim that of q")
-        num_blocks, Hkv, page, _ = k_pool.shape
         batch = total_lens.shape[0]
-        if block_table.dim() != 2 or block_table.shape[0] != batch:
-            raise ValueError("block_table must be [batch][max_blocks]")
-        out = self._out(q, out)
-        scale = lambda n, t: 0 if t is None else _tensor(n, t, torch.float32, device, (num_blocks, Hkv))  # noqa: E731
-        a = chunk_args(Shape(batch, H, Hkv, D), kv_type_of(q), kv_type_of(k_pool), page, block_table.shape[1], T,
-                       int(max_new), int(max_len), q=q.data_ptr(), q_stride=q_stride,
-                       k=_tensor("k_pool", k_pool, k_pool.dtype, device),
-                       v=_tensor("v_pool", v_pool, k_pool.dtype, device, k_pool.shape), num_blocks=num_blocks,
-                       block_table=_tensor("block_table", block_table, torch.int32, device),
-                       total_lens=_tensor("total_lens", total_lens, torch.int32, device, (batch,)),
-                       cu_new=_tensor("cu_new", cu_new, torch.int32, device, (batch + 1,)), out=out.data_ptr(),
-                       error_word=self.error_word.data_ptr(), k_scale=scale("k_scale", k_scale),
-                       v_scale=scale("v_scale", v_scale), kernel=kernel)
-        with _on(device):
-            n = paged_chunk_workspace_bytes(a)
-            workspace = torch.empty(n, dtype=torch.uint8, device=device)
-            paged_chunk_async(a, workspace.data_ptr(), n, _stream(device))
+        table, max_blocks = _table(block_table, batch, index)
+        if out is None:
+            out = q.new_empty(q.shape)
+        ks = None if k_scale is None else _tensor("k_scale", k_scale, _F32, index, pool[:2])
+        vs = None if v_scale is None else _tensor("v_scale", v_scale, _F32, index, pool[:2])
+        a = _CChunkArgs(_CShape(batch, H, pool[1], D), _type("q", q), _type("pool", k_pool), pool[2], max_blocks, T,
+                        max_new, max_len, q.data_ptr(), q_stride,
+                        _tensor("k_pool", k_pool, k_pool.dtype, index, pool),
+                        _tensor("v_pool", v_pool, k_pool.dtype, index, pool), ks, vs, pool[0], table,
+                        _tensor("total_lens", total_lens, _INT32, index, (batch,)),
+                        _tensor("cu_new", cu_new, _INT32, index, (batch + 1,)),
+                        _tensor("out", out, q.dtype, index, q.shape), self.error_word.data_ptr(), kernel)
+        self._run(a, paged_chunk_workspace_bytes, paged_chunk_async, index)
         return out
 
     def prompt(self, q, k, v, cu_lens, *, max_len: int, out=None, kernel=Kernel.auto):
         """Causal attention of packed prompts, prompt b being rows cu_lens[b] .. cu_lens[b + 1) of q, k
         and v (one type; token strides may differ), at most max_len tokens each (kvb_prompt_async)."""
-        device = self.device
-        if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:]:
+        index = self.device.index
+        if k.shape != v.shape or k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[-1]:
             raise ValueError("k and v must have one shape, with q's tokens and dim")
-        if k.dtype != q.dtype or v.dtype != q.dtype:
+        if k.dtype is not q.dtype or v.dtype is not q.dtype:
             raise ValueError("q, k and v must have one type")
-        q_stride, k_stride, v_stride = _rows("q", q, device), _rows("k", k, device), _rows("v", v, device)
+        q_stride, k_stride, v_stride = _rows("q", q, index), _rows("k", k, index), _rows("v", v, index)
         T, H, D = q.shape
-        out = self._out(q, out)
-        a = prompt_args(Shape(cu_lens.shape[0] - 1, H, k.shape[1], D), kv_type_of(q), T, int(max_len),
-                        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_stride=q_stride, k_stride=k_stride,
-                        v_stride=v_stride, cu_lens=_tensor("cu_lens", cu_lens, torch.int32, device),
-                        out=out.data_ptr(), error_word=self.error_word.data_ptr(), kernel=kernel)
-        with _on(device):
-            n = prompt_workspace_bytes(a)
-            workspace = torch.empty(n, dtype=torch.uint8, device=device)
-            prompt_async(a, workspace.data_ptr(), n, _stream(device))
+        if out is None:
+            out = q.new_empty(q.shape)
+        a = _CPromptArgs(_CShape(cu_lens.shape[0] - 1, H, k.shape[1], D), _type("q", q), T, max_len, q.data_ptr(),
+                         k.data_ptr(), v.data_ptr(), q_stride, k_stride, v_stride,
+                         _tensor("cu_lens", cu_lens, _INT32, index, (cu_lens.shape[0],)),
+                         _tensor("out", out, q.dtype, index, q.shape), self.error_word.data_ptr(), kernel)
+        self._run(a, prompt_workspace_bytes, prompt_async, index)
         return out
 
     def error_flag(self) -> int:
