@@ -987,7 +987,8 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     }
                     tc_fence_after();
                     const uint64_t k = kd + (it % NK) * (C::ITEM / 16), q = qd + t * (C::QTILE / 16);
-#pragma unroll
+                    // (rolled where the descriptors of both halves would spill)
+#pragma unroll 1
                     for (int part = 0; part < (QF32 ? 2 : 1); ++part)
 #pragma unroll
                         for (int i = 0; i < D / 16; ++i) {
@@ -999,7 +1000,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 auto values = [&](int t, uint32_t it, bool keep) {
                     const uint64_t v = vd + (it % NV) * (C::ITEM / 16);
                     const uint32_t tp = tmem + (C::ALIAS ? 128 * t : 128 * C::SBUFS + 64 * t), to = tmem + C::O_COL + D * t;
-#pragma unroll
+#pragma unroll(QF32 ? 2 : CU_ROWS / 16)
                     for (int i = 0; i < CU_ROWS / 16; ++i) {
                         const uint64_t b = v + i * (2048 / 16);
                         if constexpr (QF32) {
