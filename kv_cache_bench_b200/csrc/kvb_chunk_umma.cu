@@ -554,6 +554,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                             const float base = ref == -INFINITY ? 0.f : -ref;
                             const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
                             uint64_t l0 = 0, l1 = 0;
+                            float vs = 0.f;
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
                                 float a, b;
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                                 if (i & 2) l1 = add2(l1, pack2(a, b));
                                 else l0 = add2(l0, pack2(a, b));
                                 if constexpr (SRC == SRC_I8) {
-                                    const float vs = scales[16 + ((c0 + i) >> lp)] * vexp;
+                                    if (i % 8 == 0) vs = scales[16 + ((c0 + i) >> lp)] * vexp;  // pages of 8 tokens at least
                                     a *= vs;
                                     b *= vs;
                                     if (masked) {  // the scale of a page that this row does not see may be anything
@@ -621,6 +622,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
     #pragma unroll
                         for (int c0 = 0; c0 < CU_ROWS; c0 += 32) {
                             uint32_t pr[16];
+                            float vs = 0.f;
     #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
                                 const uint64_t x =
@@ -636,7 +638,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                                 if (i & 2) l1 = add2(l1, pack2(a, b));
                                 else l0 = add2(l0, pack2(a, b));
                                 if constexpr (SRC == SRC_I8) {
-                                    const float vs = scales[16 + ((c0 + i) >> lp)] * vexp;
+                                    if (i % 8 == 0) vs = scales[16 + ((c0 + i) >> lp)] * vexp;  // pages of 8 tokens at least
                                     a *= vs;
                                     b *= vs;
                                     if (masked) {  // the scale of a page that this row does not see may be anything
