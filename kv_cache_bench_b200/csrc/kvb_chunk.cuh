@@ -41,7 +41,7 @@ struct ChunkParams {
 };
 
 // Key tiles of 128 after which the tcgen05 kernel adds its fp32 (fp16) results' sums into `fold`.
-#define KVB_CHUNK_FOLD_F32 8
+#define KVB_CHUNK_FOLD_F32 12
 #define KVB_CHUNK_FOLD_F16 64
 
 // What a CTA of the tcgen05 kernel leaves for the merge: the unit whose first keys it took and whose others

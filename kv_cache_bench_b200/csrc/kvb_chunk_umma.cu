@@ -273,58 +273,77 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
     pdl_wait();
     pdl_trigger();
 
-    // This CTA's part of the work: the whole line's length (every thread adds up some sequences), then the
-    // sequence that the part begins in. The sums use the stages' memory, which nothing loads into yet.
-    long long* s_sum = reinterpret_cast<long long*>(smem + C::KV_OFF);
-    volatile long long* s_begin = s_sum + C::THREADS;  // sequence, place in it
-    const int per = (p.B + C::THREADS - 1) / C::THREADS;
-    const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+    // This CTA's part of the work, which the scheduler (warp 8) alone needs: the whole line's length, and the
+    // sequence that the part begins in. Up to 32 sequences are added up by that warp, more by all threads (in
+    // the stages' memory, which nothing loads into yet).
+    long long line = 0, parts = 1, first_at = 0;
+    int first_seq = p.B;
     auto seq_cost = [&](int b) {
         const ChunkSeq s = chunk_seq(p, b);
         return p.Hkv * cost_upto(p, s, seq_units(p, s));
     };
-    long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += seq_cost(b);
-    s_sum[tid] = mine;
-    if (tid == 0) s_begin[0] = p.B;
-    __syncthreads();
-    if (warp == 0) {  // exclusive sums, and the total behind them
-        long long carry = 0;
-        const int used = (p.B + per - 1) / max(per, 1);  // threads that hold sequences
-        for (int i = lane; i < (used + 31) / 32 * 32; i += 32) {
-            const long long v = s_sum[i];
-            long long x = v;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
-            }
-            s_sum[i] = carry + x - v;
-            carry += __shfl_sync(0xffffffffu, x, 31);
-        }
-        if (lane == 0) s_begin[2] = carry;
-    }
-    __syncthreads();
-    const long long line = s_begin[2];
-    const long long parts = min((long long)p.ctas, max(1ll, line / CU_COST_LEAST));
     auto part_begin = [&](long long c) { return c >= parts ? line : line * c / parts; };
-    const long long my_begin = part_begin(blockIdx.x), my_end = part_begin(blockIdx.x + 1ll);
-    if (my_begin < my_end && s_sum[tid] <= my_begin && my_begin < s_sum[tid] + mine) {
-        long long at = my_begin - s_sum[tid];
-        int b = b0;
-        for (; b < b1; ++b) {
-            const long long w = seq_cost(b);
-            if (at < w) break;
-            at -= w;
+    auto cut_line = [&]() { parts = min((long long)p.ctas, max(1ll, line / CU_COST_LEAST)); };
+    // inclusive sums over the lanes
+    auto warp_sums = [&](long long x) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
         }
-        s_begin[0] = b;
-        s_begin[1] = at;
+        return x;
+    };
+    if (p.B <= 32) {
+        if (warp == 8) {
+            const long long mine = lane < p.B ? seq_cost(lane) : 0, upto = warp_sums(mine);
+            line = __shfl_sync(0xffffffffu, upto, 31);
+            cut_line();
+            const long long at = part_begin(blockIdx.x) - (upto - mine);
+            const unsigned here = __ballot_sync(0xffffffffu, at >= 0 && at < mine);
+            if (here) {
+                first_seq = __ffs(here) - 1;
+                first_at = __shfl_sync(0xffffffffu, at, first_seq);
+            }
+        }
+    } else {
+        long long* s_sum = reinterpret_cast<long long*>(smem + C::KV_OFF);
+        volatile long long* s_begin = s_sum + C::THREADS;  // sequence, place in it, the line
+        const int per = (p.B + C::THREADS - 1) / C::THREADS, used = (p.B + per - 1) / per;
+        const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+        long long mine = 0;
+        for (int b = b0; b < b1; ++b) mine += seq_cost(b);
+        s_sum[tid] = mine;
+        if (tid == 0) s_begin[0] = p.B;
+        __syncthreads();
+        if (warp == 0) {  // exclusive sums, and the total behind them
+            long long carry = 0;
+            for (int i = lane; i < (used + 31) / 32 * 32; i += 32) {
+                const long long v = s_sum[i], x = warp_sums(v);
+                s_sum[i] = carry + x - v;
+                carry += __shfl_sync(0xffffffffu, x, 31);
+            }
+            if (lane == 0) s_begin[2] = carry;
+        }
+        __syncthreads();
+        line = s_begin[2];
+        cut_line();
+        long long at = part_begin(blockIdx.x) - s_sum[tid];
+        if (at >= 0 && at < mine) {
+            int b = b0;
+            for (; b < b1; ++b) {
+                const long long w = seq_cost(b);
+                if (at < w) break;
+                at -= w;
+            }
+            s_begin[0] = b;
+            s_begin[1] = at;
+        }
+        __syncthreads();
+        first_seq = int(s_begin[0]);
+        first_at = s_begin[1];
+        fence_proxy_async_smem();
+        __syncthreads();  // read before the stages are loaded
     }
-    __syncthreads();
-    const int first_seq = int(s_begin[0]);
-    const long long first_at = s_begin[1];
-    fence_proxy_async_smem();
-    __syncthreads();  // read before the stages are loaded
 
     // False once a wait has given up (here, or elsewhere in the CTA where this one would block).
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -452,16 +471,18 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     if (j > 0 && j % FOLD == 0) {
                         // the next product starts O anew
                         settled();
-                        const bool plain = __all_sync(0xffffffffu, older == 1.f);
-    #pragma unroll 1
-                        for (int c = 0; c < D; c += 16) {
-                            uint32_t o[16];
-                            tc_ld16(to + c, o);
+                        constexpr int FW = C::ALIAS ? 32 : 16;  // columns at a time (the scores are in registers otherwise)
+                    const bool plain = __all_sync(0xffffffffu, older == 1.f);
+#pragma unroll 1
+                        for (int c = 0; c < D; c += FW) {
+                            uint32_t o[FW];
+                            if constexpr (FW == 32) tc_ld32(to + c, o);
+                        else tc_ld16(to + c, o);
                             tc_wait_ld();
-                            pin<16>(o);
+                            pin<FW>(o);
                             float4* at = fold + (c / 4) * 128;
-    #pragma unroll
-                            for (int i = 0; i < 4; ++i, at += 128) {
+#pragma unroll
+                            for (int i = 0; i < FW / 4; ++i, at += 128) {
                                 float4 x = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
                                                        __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
                                 if (folds == 0) {
@@ -586,7 +607,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 } else {
                     // the scores move to registers at once, and their buffer is free for the next ones
                     uint32_t s[CU_ROWS];
-    #pragma unroll
+#pragma unroll
                     for (int c0 = 0; c0 < CU_ROWS; c0 += 32) tc_ld32(ts + c0, s + c0);
                     tc_wait_ld();
                     pin<CU_ROWS>(s);
@@ -595,20 +616,20 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     if (lane == 0) mbar_arrive(&s_free[t % C::SBUFS]);
                     settle_outputs();
                     if constexpr (SRC == SRC_I8) {
-    #pragma unroll
+#pragma unroll
                         for (int c = 0; c < CU_ROWS; c += 8) {
                             const float ks = scales[c >> lp];  // (pages of 128 tokens or more: one)
-    #pragma unroll
+#pragma unroll
                             for (int i = 0; i < 8; ++i) s[c + i] = __float_as_uint(__uint_as_float(s[c + i]) * ks);
                         }
                     }
                     if (masked) {
                         const int lim = limit - k0;
-    #pragma unroll
+#pragma unroll
                         for (int c0 = 0; c0 < CU_ROWS; c0 += 32) {
                             // one bit a key, so that a few instructions make the predicates
                             const uint32_t sees = lim - c0 >= 32 ? ~0u : lim - c0 <= 0 ? 0u : (1u << (lim - c0)) - 1u;
-    #pragma unroll
+#pragma unroll
                             for (int c = 0; c < 32; ++c)
                                 if (!(sees >> c & 1u)) s[c0 + c] = 0xff800000u;  // -inf
                         }
@@ -619,11 +640,11 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                         const float base = ref == -INFINITY ? 0.f : -ref;
                         const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
                         uint64_t l0 = 0, l1 = 0;
-    #pragma unroll
+#pragma unroll
                         for (int c0 = 0; c0 < CU_ROWS; c0 += 32) {
                             uint32_t pr[16];
                             float vs = 0.f;
-    #pragma unroll
+#pragma unroll
                             for (int i = 0; i < 32; i += 2) {
                                 const uint64_t x =
                                     fma2(pack2(__uint_as_float(s[c0 + i]), __uint_as_float(s[c0 + i + 1])), f2, b2);
@@ -663,7 +684,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     for (;;) {
                         if (raise) {
                             float m0 = -INFINITY, m1 = -INFINITY;
-    #pragma unroll
+#pragma unroll
                             for (int i = 0; i < CU_ROWS; i += 4) {
                                 m0 = max3_nan(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
                                 m1 = max3_nan(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
@@ -820,7 +841,8 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 ++published;
             };
             ChunkPiece piece{0, 0, 0, -1, 0};
-            long long place = my_begin, at = first_at;  // on the line; in the sequence
+            const long long my_end = part_begin(blockIdx.x + 1ll);
+            long long place = part_begin(blockIdx.x), at = first_at;  // on the line; in the sequence
             ChunkSeq s{};
             int units = 0;
             long long w = 0;  // cost of one KV head of sequence b

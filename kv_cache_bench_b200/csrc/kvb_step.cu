@@ -251,14 +251,17 @@ __device__ __forceinline__ float amax4(float4 v) {
 constexpr int AP_REGS = 16;
 
 template <typename SRC, int TPR>
-__global__ void __launch_bounds__(AP_THREADS) append_i8_kernel(const AppendParams p, int tpg) {
+__global__ void __launch_bounds__(AP_THREADS, 3) append_i8_kernel(const AppendParams p, int tpg,
+                                                                int heads) {
     constexpr int WARPS = TPR / 32;
     __shared__ int s_tok[AP_THREADS], s_n[AP_THREADS], s_at[AP_THREADS];  // a CTA-wide group's runs
     __shared__ long long s_block[AP_THREADS];
     __shared__ int s_runs;
     __shared__ float s_max[2][AP_THREADS / 32];
     const int lane = threadIdx.x & 31, gl = threadIdx.x % TPR;
-    const long long tok0 = ((long long)blockIdx.x * (AP_THREADS / TPR) + threadIdx.x / TPR) * tpg;
+    // The heads of a token group are neighbours in the grid, so that CTAs that run together read whole rows.
+    const int by = int(blockIdx.x % heads);
+    const long long tok0 = ((long long)(blockIdx.x / heads) * (AP_THREADS / TPR) + threadIdx.x / TPR) * tpg;
     pdl_wait();
     pdl_trigger();
     // each of the first tpg threads of a group decodes one token
@@ -279,7 +282,7 @@ __global__ void __launch_bounds__(AP_THREADS) append_i8_kernel(const AppendParam
             if (c0 >= 0 && c0 <= t) {
                 if (start < 0 || (long long)total > (long long)p.max_blocks * p.page) {
                     // -1 marks a sequence that the plan refused: it was reported there
-                    if (total != -1 && t == c0 && blockIdx.y == 0 && p.error_flag)
+                    if (total != -1 && t == c0 && by == 0 && p.error_flag)
                         raise_error(p.error_flag, KVB_DEVERR_LENGTH);
                 } else {
                     const int pos = int(start) + (t - c0), pg = kvb_div(pos, p.div_page);
@@ -289,7 +292,7 @@ __global__ void __launch_bounds__(AP_THREADS) append_i8_kernel(const AppendParam
                         if (id >= 0 && id < p.num_blocks) {
                             block = id;
                             n = min(p.page - at, c1 - t);
-                        } else if (blockIdx.y == 0 && p.error_flag) {
+                        } else if (by == 0 && p.error_flag) {
                             raise_error(p.error_flag, KVB_DEVERR_BLOCK);
                         }
                     }
@@ -384,7 +387,7 @@ __global__ void __launch_bounds__(AP_THREADS) append_i8_kernel(const AppendParam
             s_tok[i] = t, s_n[i] = n, s_at[i] = at, s_block[i] = block;
         }
         __syncthreads();
-        for (int y = blockIdx.y; y < 2 * p.Hkv; y += gridDim.y)
+        for (int y = by; y < 2 * p.Hkv; y += heads)
             for (int i = 0; i < s_runs; ++i) run(y, s_tok[i], s_n[i], s_at[i], s_block[i]);
     } else {
         for (unsigned runs = __ballot_sync(0xffffffffu, block >= 0); runs; runs &= runs - 1) {
@@ -392,7 +395,7 @@ __global__ void __launch_bounds__(AP_THREADS) append_i8_kernel(const AppendParam
             const int rt = __shfl_sync(0xffffffffu, t, l), rn = __shfl_sync(0xffffffffu, n, l);
             const int rat = __shfl_sync(0xffffffffu, at, l);
             const long long rblock = __shfl_sync(0xffffffffu, block, l);
-            for (int y = blockIdx.y; y < 2 * p.Hkv; y += gridDim.y) run(y, rt, rn, rat, rblock);
+            for (int y = by; y < 2 * p.Hkv; y += heads) run(y, rt, rn, rat, rblock);
         }
     }
 }
@@ -424,11 +427,12 @@ cudaError_t launch_i8(const AppendParams& p, int num_sms, cudaStream_t stream) {
         while (tpg < 32 && (long long)p.num_tokens / tpg * p.Hkv * 2 > (long long)num_sms * 64) tpg *= 2;
     const long long groups = ((long long)p.num_tokens + tpg - 1) / tpg, per = cta ? 1 : AP_THREADS / 32;
     cudaLaunchConfig_t cfg = {};
-    // heads of K and V side by side, as many as make four CTAs an SM (the others follow in the same CTA, which
-    // knows its runs already)
+    // heads of K and V side by side, as many as make six CTAs an SM; a CTA does the others after them, with the
+    // runs that it found once
     const long long x = (groups + per - 1) / per;
-    const long long y = std::min<long long>(2ll * p.Hkv, std::max<long long>(1, (4ll * num_sms + x - 1) / x));
-    cfg.gridDim = dim3((unsigned)x, (unsigned)y);
+    const long long y = std::min<long long>(2ll * p.Hkv, std::max<long long>(1, (6ll * num_sms + x - 1) / x));
+    if (x * y >= (1ll << 31)) return cudaErrorInvalidConfiguration;
+    cfg.gridDim = dim3((unsigned)(x * y));
     cfg.blockDim = dim3(AP_THREADS);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -436,8 +440,8 @@ cudaError_t launch_i8(const AppendParams& p, int num_sms, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cta ? cudaLaunchKernelEx(&cfg, append_i8_kernel<SRC, AP_THREADS>, p, tpg)
-               : cudaLaunchKernelEx(&cfg, append_i8_kernel<SRC, 32>, p, tpg);
+    return cta ? cudaLaunchKernelEx(&cfg, append_i8_kernel<SRC, AP_THREADS>, p, tpg, int(y))
+               : cudaLaunchKernelEx(&cfg, append_i8_kernel<SRC, 32>, p, tpg, int(y));
 }
 
 }  // namespace
