@@ -273,19 +273,17 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
     pdl_wait();
     pdl_trigger();
 
-    // This CTA's part of the work, which the scheduler (warp 8) alone needs: the whole line's length, and the
-    // sequence that the part begins in. Up to 32 sequences are added up by that warp, more by all threads (in
-    // the stages' memory, which nothing loads into yet).
-    long long line = 0, parts = 1, first_at = 0;
-    int first_seq = p.B;
+    // This CTA's part of the work: the whole line's length, and the sequence that the part begins in. Up to 32
+    // sequences are added up by one warp, more by all threads. (In the stages' memory, which nothing loads
+    // into yet.)
+    long long* s_sum = reinterpret_cast<long long*>(smem + C::KV_OFF);
+    volatile long long* s_begin = s_sum + C::THREADS;  // sequence, place in it, the line
     auto seq_cost = [&](int b) {
         const ChunkSeq s = chunk_seq(p, b);
         return p.Hkv * cost_upto(p, s, seq_units(p, s));
     };
-    auto part_begin = [&](long long c) { return c >= parts ? line : line * c / parts; };
-    auto cut_line = [&]() { parts = min((long long)p.ctas, max(1ll, line / CU_COST_LEAST)); };
-    // inclusive sums over the lanes
-    auto warp_sums = [&](long long x) {
+    auto parts_of = [&](long long line) { return min((long long)p.ctas, max(1ll, line / CU_COST_LEAST)); };
+    auto warp_sums = [&](long long x) {  // inclusive, over the lanes
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long y = __shfl_up_sync(0xffffffffu, x, o);
@@ -294,20 +292,21 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
         return x;
     };
     if (p.B <= 32) {
-        if (warp == 8) {
+        if (warp == 0) {
             const long long mine = lane < p.B ? seq_cost(lane) : 0, upto = warp_sums(mine);
-            line = __shfl_sync(0xffffffffu, upto, 31);
-            cut_line();
-            const long long at = part_begin(blockIdx.x) - (upto - mine);
-            const unsigned here = __ballot_sync(0xffffffffu, at >= 0 && at < mine);
-            if (here) {
-                first_seq = __ffs(here) - 1;
-                first_at = __shfl_sync(0xffffffffu, at, first_seq);
+            const long long total = __shfl_sync(0xffffffffu, upto, 31), n = parts_of(total);
+            const long long at = (blockIdx.x >= n ? total : total * blockIdx.x / n) - (upto - mine);
+            if (lane == 0) {
+                s_begin[0] = p.B;
+                s_begin[2] = total;
+            }
+            __syncwarp();
+            if (at >= 0 && at < mine) {
+                s_begin[0] = lane;
+                s_begin[1] = at;
             }
         }
     } else {
-        long long* s_sum = reinterpret_cast<long long*>(smem + C::KV_OFF);
-        volatile long long* s_begin = s_sum + C::THREADS;  // sequence, place in it, the line
         const int per = (p.B + C::THREADS - 1) / C::THREADS, used = (p.B + per - 1) / per;
         const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
         long long mine = 0;
@@ -325,9 +324,8 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             if (lane == 0) s_begin[2] = carry;
         }
         __syncthreads();
-        line = s_begin[2];
-        cut_line();
-        long long at = part_begin(blockIdx.x) - s_sum[tid];
+        const long long total = s_begin[2], n = parts_of(total);
+        long long at = (blockIdx.x >= n ? total : total * blockIdx.x / n) - s_sum[tid];
         if (at >= 0 && at < mine) {
             int b = b0;
             for (; b < b1; ++b) {
@@ -338,12 +336,15 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             s_begin[0] = b;
             s_begin[1] = at;
         }
-        __syncthreads();
-        first_seq = int(s_begin[0]);
-        first_at = s_begin[1];
-        fence_proxy_async_smem();
-        __syncthreads();  // read before the stages are loaded
     }
+    __syncthreads();
+    const long long line = s_begin[2], parts = parts_of(line);
+    auto part_begin = [&](long long c) { return c >= parts ? line : line * c / parts; };
+    const long long my_begin = part_begin(blockIdx.x), my_end = part_begin(blockIdx.x + 1ll);
+    const int first_seq = int(s_begin[0]);
+    const long long first_at = s_begin[1];
+    fence_proxy_async_smem();
+    __syncthreads();  // read before the stages are loaded
 
     // False once a wait has given up (here, or elsewhere in the CTA where this one would block).
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -841,8 +842,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 ++published;
             };
             ChunkPiece piece{0, 0, 0, -1, 0};
-            const long long my_end = part_begin(blockIdx.x + 1ll);
-            long long place = part_begin(blockIdx.x), at = first_at;  // on the line; in the sequence
+            long long place = my_begin, at = first_at;  // on the line; in the sequence
             ChunkSeq s{};
             int units = 0;
             long long w = 0;  // cost of one KV head of sequence b
