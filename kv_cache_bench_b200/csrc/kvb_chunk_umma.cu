@@ -542,7 +542,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                                 if (!(sees >> c & 1u)) s[c] = 0xff800000u;  // -inf
                         }
                         float part = 0.f, top = 0.f;
-                        bool raise = j == 0 && c0 == 0;
+                        bool raise = j == 0 && c0 == 0, need = raise;  // some row of the warp's; this row
                         for (;;) {
                             if (raise) {
                                 float m0 = -INFINITY, m1 = -INFINITY;
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                                 top = fmaxf_nan(m0, m1) * f;
                                 const float up = ceilf(top) - CU_SHIFT;
                                 float scale = 1.f;
-                                if (up > ref) {
+                                if (need && up > ref) {
                                     scale = ref == -INFINITY ? 0.f : ex2(ref - up);
                                     ref = up;
                                     l *= scale;
@@ -599,7 +599,8 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                             float a, b;
                             unpack2(add2(l0, l1), a, b);
                             part = a + b;
-                            if (raise || !__any_sync(0xffffffffu, !(part <= CU_MOST))) break;
+                            need = live && !(part <= CU_MOST);
+                            if (raise || !__any_sync(0xffffffffu, need)) break;
                             raise = true;
                         }
                         tc_st32(tp + c0, pr);
@@ -681,7 +682,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     // highest score, O and l follow, and the probabilities are computed with that. (One copy of
                     // their code: the SM's instruction cache holds little more than the loop.)
                     float top = 0.f;
-                    bool raise = j == 0;
+                    bool raise = j == 0, need = raise;  // some row of the warp's; this row
                     for (;;) {
                         if (raise) {
                             float m0 = -INFINITY, m1 = -INFINITY;
@@ -692,7 +693,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                             }
                             top = fmaxf_nan(m0, m1) * f - CU_SHIFT;
                             float scale = 1.f;
-                            if (top > ref) {
+                            if (need && top > ref) {
                                 scale = ref == -INFINITY ? 0.f : ex2(ref - top);
                                 ref = top;
                                 l *= scale;
@@ -700,7 +701,10 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                             if (j > 0) rescale(scale);
                         }
                         sum = probabilities();
-                        if (raise || !__any_sync(0xffffffffu, !(sum <= CU_MOST))) break;
+                        // (rows of no token hold anything: they do not count, and a row's result does not
+                        // depend on its neighbours)
+                        need = live && !(sum <= CU_MOST);
+                        if (raise || !__any_sync(0xffffffffu, need)) break;
                         raise = true;
                     }
                     if (!(top < INFINITY)) sum = __int_as_float(0x7fc00000);  // a NaN or +inf score: the row is NaN

@@ -242,6 +242,56 @@ def test_a_request_served_step_by_step(qt, kv):
         lens, ring_pos = p.total_lens, p.ring_pos
 
 
+@pytest.mark.parametrize("qt,kv", [(F16, F16), (F16, I8), (F32, F16), (F32, I8)])
+@pytest.mark.parametrize("H,Hkv", [(20, 4), (7, 1), (33, 11)])
+def test_results_do_not_depend_on_what_ran_before(qt, kv, H, Hkv):
+    """Group sizes that leave rows of the query tile without a token; calls with other values in between."""
+    new, ctx = [3, 97, 1, 40], [700, 30, 0, 2500]
+    c = make_cache(new, ctx, Hkv, 128, 32, kv, 3)
+    q, other = make_q(sum(new), H, 128, qt, 4) * 8, make_q(500, H, 128, qt, 5) * 60
+    x = make_cache([500], [40], Hkv, 128, 32, kv, 6)
+    a = ops.PagedPrefill()
+
+    def run():
+        return a.chunk(q, c["k"], c["v"], c["table"], ints(c["total"]), starts(new), max_new=97, max_len=2540,
+                       k_scale=c["ks"], v_scale=c["vs"])
+
+    first = run()
+    for _ in range(10):
+        a.chunk(other, x["k"], x["v"], x["table"], ints(x["total"]), starts([500]), max_new=500, max_len=540,
+                k_scale=x["ks"], v_scale=x["vs"])
+        assert torch.equal(run(), first)
+
+
+@pytest.mark.parametrize("kv", [F16, I8])
+def test_pools_past_32_bits(kv):
+    """Pages whose first value lies more than 2^31 elements into the pool (and 2^32 bytes)."""
+    Hkv, D, page, num_blocks = 8, 128, 128, 18000
+    pools = [torch.zeros(num_blocks, Hkv, page, D, dtype=kv, device="cuda") for _ in range(2)]
+    scales = [torch.zeros(num_blocks, Hkv, device="cuda") for _ in range(2)]
+    assert pools[0].numel() > 1 << 31
+    new, ids = [200, 129], [[num_blocks - 1, num_blocks - 7], [num_blocks - 3, 5]]
+    table = ints(ids)
+    T = sum(new)
+    q, k, v = make_q(T, 16, D, F16, 1), make_q(T, Hkv, D, F16, 2), make_q(T, Hkv, D, F16, 3)
+    total, cu = ints(new), starts(new)
+    if kv is I8:
+        ops.append_kv_i8(k, v, *pools, *scales, block_table=table, total_lens=total, cu_new=cu)
+    else:
+        slots = [ids[b][p // page] * page + p % page for b, n in enumerate(new) for p in range(n)]
+        ops.append_kv(k, v, *pools, slot_map=ints(slots, torch.int64))
+    a = ops.PagedPrefill()
+    for kernel in (AUTO, SIMT):
+        o = a.chunk(q, *pools, table, total, cu, max_new=200, max_len=200, k_scale=scales[0] if kv is I8 else None,
+                    v_scale=scales[1] if kv is I8 else None, kernel=kernel)
+        assert a.error_flag() == 0
+        for b, (x, n) in enumerate(zip(cu.tolist(), new)):
+            c = dict(total=new, page=page, table=table, k=pools[0], v=pools[1], ks=scales[0] if kv is I8 else None,
+                     vs=scales[1] if kv is I8 else None)
+            want = attention64(q[x:x + n], rows_of(c, "k", b), rows_of(c, "v", b), 0)
+            assert (o[x:x + n].double() - want).abs().max().item() <= tolerance(F16)
+
+
 @pytest.mark.parametrize("qt,kv", [(F16, F16), (F16, I8), (F32, F16)])
 def test_captured_steps_on_another_stream(qt, kv):
     """Two captured calls that share the object, replayed at once on two streams, and an eager call."""
