@@ -434,6 +434,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 }
             }
             float ref = -INFINITY;  // probabilities are 2^(f s - ref)
+            const float most = live ? CU_MOST : INFINITY;  // rows of no token hold anything: they move no reference
             float l = 0.f;
             float vexp = 0.f;       // int8: 2^-e, probabilities times the value scales times this; 0: not set
             float older = 1.f;      // what the folded sum has to be scaled by
@@ -542,7 +543,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                                 if (!(sees >> c & 1u)) s[c] = 0xff800000u;  // -inf
                         }
                         float part = 0.f, top = 0.f;
-                        bool raise = j == 0 && c0 == 0, need = raise;  // some row of the warp's; this row
+                        bool raise = j == 0 && c0 == 0;
                         for (;;) {
                             if (raise) {
                                 float m0 = -INFINITY, m1 = -INFINITY;
@@ -554,7 +555,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                                 top = fmaxf_nan(m0, m1) * f;
                                 const float up = ceilf(top) - CU_SHIFT;
                                 float scale = 1.f;
-                                if (need && up > ref) {
+                                if (up > ref) {
                                     scale = ref == -INFINITY ? 0.f : ex2(ref - up);
                                     ref = up;
                                     l *= scale;
@@ -599,8 +600,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                             float a, b;
                             unpack2(add2(l0, l1), a, b);
                             part = a + b;
-                            need = live && !(part <= CU_MOST);
-                            if (raise || !__any_sync(0xffffffffu, need)) break;
+                            if (raise || !__any_sync(0xffffffffu, part > most)) break;
                             raise = true;
                         }
                         tc_st32(tp + c0, pr);
@@ -678,11 +678,11 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                         return a + b;
                     };
                     // With the reference so far first. No probability is above their sum, so a sum in bounds needs
-                    // no maximum. Otherwise (NaN included, and at the first key tile) the reference rises to the
+                    // no maximum (a NaN makes the row NaN as it is). Otherwise, and at the first key tile, the reference rises to the
                     // highest score, O and l follow, and the probabilities are computed with that. (One copy of
                     // their code: the SM's instruction cache holds little more than the loop.)
                     float top = 0.f;
-                    bool raise = j == 0, need = raise;  // some row of the warp's; this row
+                    bool raise = j == 0;
                     for (;;) {
                         if (raise) {
                             float m0 = -INFINITY, m1 = -INFINITY;
@@ -693,7 +693,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                             }
                             top = fmaxf_nan(m0, m1) * f - CU_SHIFT;
                             float scale = 1.f;
-                            if (need && top > ref) {
+                            if (top > ref) {
                                 scale = ref == -INFINITY ? 0.f : ex2(ref - top);
                                 ref = top;
                                 l *= scale;
@@ -701,10 +701,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                             if (j > 0) rescale(scale);
                         }
                         sum = probabilities();
-                        // (rows of no token hold anything: they do not count, and a row's result does not
-                        // depend on its neighbours)
-                        need = live && !(sum <= CU_MOST);
-                        if (raise || !__any_sync(0xffffffffu, need)) break;
+                        if (raise || !__any_sync(0xffffffffu, sum > most)) break;
                         raise = true;
                     }
                     if (!(top < INFINITY)) sum = __int_as_float(0x7fc00000);  // a NaN or +inf score: the row is NaN
