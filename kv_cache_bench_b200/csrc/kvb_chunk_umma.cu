@@ -6,9 +6,10 @@
 // serves the whole group; a unit is two query tiles and 128-key tiles of their keys. Per key tile
 //     S[128 rows x 128 keys] = Q K^T      (Q, K in shared memory, K-major)
 //     P = exp2(f S - m), l += row sums
-//     O[128 rows x D] += P V              (P in tensor memory over S, V in shared memory, MN-major)
-// with the running reference m of a row raised only when a score passes it by 2^8 (then O and l are
-// scaled in place), so O stays in tensor memory. One persistent CTA per SM, 16 warps:
+//     O[128 rows x D] += P V              (P in tensor memory, V in shared memory, MN-major)
+// with the running reference m of a row raised only when a tile's probabilities sum to more than 2^14 (then O
+// and l are scaled in place), so O stays in tensor memory and the common tile needs no maximum. One
+// persistent CTA per SM, 16 warps:
 //   0-3, 4-7   softmax of query tiles 0 and 1, one thread per row (tensor-memory lane).
 //   8          unit scheduler, and TMA producer of the key tiles and the query tiles.
 //   9          TMA producer of the value tiles (with small pages one warp's issue of 16 boxes a tile was slower
@@ -23,6 +24,14 @@
 //              converted to fp16 (exact); the scales are applied to the scores and to the probabilities.
 // fp32 queries (QF32) keep fp32-level results: q and p are split as fp16(x) + fp16(x - fp16(x)) (about 22
 // bits; q prescaled per row by a power of two) and both products run on both halves.
+//
+// What bounds it: at head dim 128 the four products of a pair of query tiles take 2048 cycles a key tile and
+// the exponentials as many, and under load the 1 kW power cap lowers the clock, so that the cap on sustained
+// library products (1375 of 1653 TFLOP/s) is the mark. A prompt of 8192 tokens (32 heads over 8, 0.55 TFLOP
+// that count): 445 us, 1240 TFLOP/s; 2048 tokens on a 32 k context: 920 us, 1160 TFLOP/s; 512 fp32 queries on
+// 32 k of int8 pages: 609 us, 900 TFLOP/s of the products with split operands. Few tokens on long contexts are
+// bound by memory and by the loads in flight (8 ragged chunks, 311 MB: 75 us, 4.1 TB/s) and, at the smallest, by
+// the start, first loads and the join (4 x 3-8 tokens on 4 k, 57 MB: 28 us).
 #include <cuda.h>
 #include <cuda_fp16.h>
 
@@ -38,22 +47,33 @@ using namespace kvb_dev;
 constexpr int CU_ROWS = 128;            // query rows of a tile, keys of a tile
 constexpr int CU_SUB = CU_ROWS * 128;   // bytes of [128 rows][128 B], one 128-byte-swizzled slice
 constexpr int CU_RING = 2;              // units in flight between the roles
-constexpr int CU_POLY = 0, CU_POLY_OF = 4;  // pairs of probabilities on the FMA pipe, of so many
+// One pair of probabilities in so many is computed on the FMA pipe instead of the exponential unit. At head dim
+// 64 the products are half as long and the exponentials are what a tile takes (prompt of 8192 tokens: 464 us
+// without, 439 with one in 8, 446 in 4, 513 in 2); at 128 the products are, and it costs (444 -> 439, but 2048
+// tokens on 32 k 948 -> 983).
+template <int D>
+constexpr int CU_POLY_OF = D == 64 ? 8 : 0;
 constexpr int CU_CLEAN = 8;             // value tiles on their way to the cleaning warps: at most their stages are
 enum { SRC_F16 = 0, SRC_I8 = 1, SRC_PACKED = 2 };
 // The tensor cores add into O with truncation, an error of up to 2^-23 of O per product of 16 keys and in
 // one direction. So O is added into an fp32 sum in the workspace (rounded to nearest) and started anew
-// every so many key tiles: often for fp32 results, rarely for fp16 ones.
+// every so many key tiles: often for fp32 results, rarely for fp16 ones. (512 fp32 queries on 32 k int8:
+// relative error 3.5e-5 and 3.5e-6 for the plain fp32 form; folded every 8, 12, 16 tiles 3.6e-6, 4.5e-6,
+// 5.6e-6 and 647, 609, 605 us.)
 constexpr int CU_FOLD_F32 = KVB_CHUNK_FOLD_F32, CU_FOLD_F16 = KVB_CHUNK_FOLD_F16;
-constexpr float CU_SHIFT = 5.f;  // a row's highest score so far has probability 2^CU_SHIFT: small ones stay normal in fp16
+// A row's highest score at its reference's last move has probability 2^CU_SHIFT, so that small ones stay normal
+// in fp16.
+constexpr float CU_SHIFT = 5.f;
 constexpr float CU_MOST = 16384.f;  // a key tile's probabilities of a row may sum to this before the reference moves
 
 // The work of a call is a line: sequence by sequence, KV head by KV head, unit by unit, each unit as long as
 // its cost (keys, and an overhead), cut into equal parts, one per CTA. So every CTA ends at about the same
 // time whatever the lengths, and a call with few units splits their keys. A unit that a cut goes through
-// (at a key tile) is computed in pieces, which a second small kernel joins. Costs are in quarter keys: a
-// unit with one query tile counts three quarters.
-constexpr long long CU_COST_UNIT = 4 * 480;       // a unit's overhead
+// (at a key tile) is computed in pieces, which a second small kernel joins. (Whole units handed out longest
+// first, their keys split evenly only where units were fewer than SMs: 250 us instead of 112 for 8 chunks of
+// 1-256 tokens on contexts of 512-30000, and 948 instead of 923 for 2048 tokens on 32 k.) Costs are in quarter
+// keys: a unit with one query tile counts three quarters.
+constexpr long long CU_COST_UNIT = 4 * 480;       // a unit's overhead: its queries' load, first maximum, output
 constexpr long long CU_COST_LEAST = 4 * 512;      // work that is worth a CTA
 constexpr int CU_SNAP = 2;                        // no cut nearer than this to a unit's first or last key tile
 
@@ -651,7 +671,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                                 const uint64_t x =
                                     fma2(pack2(__uint_as_float(s[c0 + i]), __uint_as_float(s[c0 + i + 1])), f2, b2);
                                 float a, b;
-                                if ((i / 2) % CU_POLY_OF < CU_POLY) {
+                                if (CU_POLY_OF<D> > 0 && i / 2 % std::max(CU_POLY_OF<D>, 1) == 0) {
                                     exp2_poly2(x, a, b);
                                 } else {
                                     unpack2(x, a, b);
@@ -678,9 +698,9 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                         return a + b;
                     };
                     // With the reference so far first. No probability is above their sum, so a sum in bounds needs
-                    // no maximum (a NaN makes the row NaN as it is). Otherwise, and at the first key tile, the reference rises to the
-                    // highest score, O and l follow, and the probabilities are computed with that. (One copy of
-                    // their code: the SM's instruction cache holds little more than the loop.)
+                    // no maximum (a NaN makes the row NaN as it is). Otherwise, and at the first key tile, the
+                    // reference rises to the highest score, O and l follow, and the probabilities are computed
+                    // with that. (One copy of their code: the instruction cache holds little more than the loop.)
                     float top = 0.f;
                     bool raise = j == 0;
                     for (;;) {
