@@ -43,6 +43,6 @@ struct AppendParams {
     unsigned* error_flag;     // or null
     long long num_blocks;
     int num_tokens, B, Hkv, D, page, max_blocks;
-    KvbDiv div_page, div_row, div_token;  // page; 16-byte (int8: four-value) pieces of a row, of a token
+    KvbDiv div_page, div_row;  // page; pieces of a row (16 pool bytes; int8: four values)
 };
 cudaError_t kvb_launch_append(const AppendParams& p, int src_type, int kv_type, int num_sms, cudaStream_t stream);

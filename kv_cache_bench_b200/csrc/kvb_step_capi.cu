@@ -346,7 +346,6 @@ int kvb_paged_append(const kvb_append_args* a, void* stream) {
     p.max_blocks = a->max_blocks;
     p.div_page = kvb_div_make((uint32_t)a->page_size);
     p.div_row = kvb_div_make((uint32_t)(i8 ? s.head_dim / 4 : s.head_dim * elem_size(a->kv_type) / 16));
-    p.div_token = kvb_div_make(p.div_row.d * (uint32_t)s.num_kv_heads);
     int sms = 0;
     if (int rc = kvb_device_sms(&sms)) return rc;
     return launched(kvb_launch_append(p, a->src_type, a->kv_type, sms, static_cast<cudaStream_t>(stream)));
