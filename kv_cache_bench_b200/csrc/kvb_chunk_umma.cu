@@ -493,13 +493,13 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     if (j > 0 && j % FOLD == 0) {
                         // the next product starts O anew
                         settled();
-                        constexpr int FW = C::ALIAS ? 32 : 16;  // columns at a time (the scores are in registers otherwise)
-                    const bool plain = __all_sync(0xffffffffu, older == 1.f);
+                        constexpr int FW = C::ALIAS ? 32 : 16;  // columns at a time (16 beside a tile's scores)
+                        const bool plain = __all_sync(0xffffffffu, older == 1.f);
 #pragma unroll 1
                         for (int c = 0; c < D; c += FW) {
                             uint32_t o[FW];
                             if constexpr (FW == 32) tc_ld32(to + c, o);
-                        else tc_ld16(to + c, o);
+                            else tc_ld16(to + c, o);
                             tc_wait_ld();
                             pin<FW>(o);
                             float4* at = fold + (c / 4) * 128;

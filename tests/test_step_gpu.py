@@ -128,6 +128,34 @@ def test_plan_reports_bad_ids_and_a_bad_ring():
                    table=np.array([[6], [-7]], np.int32))
 
 
+def test_pages_go_round():
+    """Requests come and go for many steps on a small ring: no live page is ever handed out twice, and every
+    page comes back."""
+    rng = np.random.default_rng(0)
+    B, page, num_blocks, width = 5, 4, 30, 9
+    ring = ints(rng.permutation(num_blocks))
+    pos = ints([0, num_blocks], torch.int64)
+    table = torch.full((B, width), -1, dtype=torch.int32, device="cuda")
+    lens, err = ints([0] * B), ints([0])
+    for step in range(60):
+        room = width * page - lens.cpu().numpy()
+        new = np.minimum(rng.integers(0, 9, B), room)
+        p = ops.plan_step(lens, ints(new), table, ring, pos, page_size=page, num_blocks=num_blocks,
+                          num_tokens=int(new.sum()), error_word=err)
+        lens, pos = torch.where(p.total_lens < 0, lens, p.total_lens), p.ring_pos
+        b = int(rng.integers(0, B))
+        if rng.random() < 0.5:  # request b ends
+            pages = -(-int(lens[b]) // page)
+            ring[(pos[1] + torch.arange(pages, device="cuda")) % num_blocks] = table[b, :pages]
+            pos[1] += pages
+            lens[b] = 0
+        owned = [table[i, j].item() for i in range(B) for j in range(-(-int(lens[i]) // page))]
+        head, tail = pos.tolist()
+        free = ring[torch.arange(head, tail, device="cuda") % num_blocks].tolist()
+        assert sorted(owned + free) == list(range(num_blocks)), step
+    assert pos[0].item() > num_blocks and err.item() in (0, 2)
+
+
 # ---- append -----------------------------------------------------------------------------------------
 
 def source(T, Hkv, D, dtype, seed, pad=0):
