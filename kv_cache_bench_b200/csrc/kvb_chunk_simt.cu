@@ -426,7 +426,9 @@ cudaError_t kvb_launch_chunk_merge(const ChunkParams& p, int q_type, int D, int 
 
 cudaError_t kvb_launch_chunk_join(const ChunkParams& p, int q_type, int D, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)p.ctas, 8);
+    // 32 rows a CTA; where no sequence fills a query tile, only the rows that can hold a token
+    const int rows = p.max_new <= p.tile_tokens ? p.max_new * p.G : 256;
+    cfg.gridDim = dim3((unsigned)p.ctas, (unsigned)((rows + 31) / 32));
     cfg.blockDim = dim3(256);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
