@@ -120,15 +120,16 @@ struct CCfg {
     static constexpr int SBUFS = ALIAS || D == 64 ? 2 : 1;    // score buffers: the tiles', or one that they share
     static constexpr int O_COL = ALIAS ? 256 : 128 * SBUFS + 128;
     static_assert(O_COL + 2 * D <= 512, "tensor memory");
-    // int8: key tiles whose scales are kept. A tile's are written when the keys RAWS + NK tiles before it are
-    // through their score products; a softmax may then still be reading those of the tile before.
-    static constexpr int SR = QF32 && D == 128 ? 4 : 8;
-    static_assert(RAWS + NK + 2 <= SR, "scale ring");
+    // int8: key tiles whose scales are kept, enough that the ring holds no key tile up. (A query tile can fall
+    // several key tiles behind the other one, over units that only that one has rows in, so a slot is
+    // written when both are through with what it held.)
+    static constexpr int SR = SRC != SRC_I8 ? 0 : QF32 && D == 128 ? 4 : 8;
+    static_assert(SRC != SRC_I8 || RAWS + NK + 2 <= SR, "scale ring");
     static constexpr size_t Q_OFF = 0;
     static constexpr size_t KV_OFF = 2 * QTILE;
     static constexpr size_t RAW_OFF = KV_OFF + size_t(STAGES) * ITEM;  // (K's stages, then V's)
     static constexpr size_t BAR_OFF = RAW_OFF + size_t(2 * RAWS) * RAW;
-    static constexpr int NBARS = 2 * STAGES + 4 * RAWS + 11 + CU_CLEAN + 2 * CU_RING;
+    static constexpr int NBARS = 2 * STAGES + 4 * RAWS + 11 + CU_CLEAN + 2 * CU_RING + SR;
     static constexpr size_t UNIT_OFF = kvb_align_up(BAR_OFF + 8 * NBARS, 64);
     static constexpr size_t SCALE_OFF = UNIT_OFF + 64 * CU_RING;           // [SR tiles][K, V][16 pages]
     static constexpr size_t VMAX_OFF = SCALE_OFF + (RAWS ? SR * 2 * 16 * 4 : 0);  // [SR tiles]
@@ -257,6 +258,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
     uint64_t* dirty_full = pv_done + 2;   // [CU_CLEAN] a value tile loaded that passes the cleaning warps first
     uint64_t* r_full = dirty_full + CU_CLEAN;  // [CU_RING] unit published
     uint64_t* r_empty = r_full + CU_RING;
+    uint64_t* sc_free = r_empty + CU_RING;  // [SR] int8: both softmax groups are through with the slot's scales
     auto ring = [&](int e) -> RingUnit& { return *reinterpret_cast<RingUnit*>(smem + C::UNIT_OFF + 64 * (e % CU_RING)); };
     float* s_scale = reinterpret_cast<float*>(smem + C::SCALE_OFF);
     float* s_vmax = reinterpret_cast<float*>(smem + C::VMAX_OFF);
@@ -273,6 +275,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             else if (b >= rk_empty && b < q_full) n = C::HELPERS / 2;
             else if (b >= q_full && b < q_empty) n = QF32 ? C::SOFT / 2 : 1;
             else if (b >= s_free && b < pv_done) n = C::SOFT / 2;
+            else if (b >= sc_free) n = C::SOFT;
             else if (b >= r_empty) n = (C::ALIAS ? 2 : 3) + C::SOFT + C::HELPERS;  // V producer, issuers, the rest
             mbar_init(b, n);
         }
@@ -400,6 +403,19 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&r_empty[e % CU_RING]);
             };
+            // The unit's key tiles from j on, which only the other query tile has. (One turn of the ring at a
+            // time: an arrival counts for the phase that is open.)
+            auto pass = [&](int j) {
+                if constexpr (SRC == SRC_I8) {
+                    for (; j < nall && !stop(); ++j) {
+                        const uint32_t i = tiles + j;
+                        if (i >= C::SR) wait(&sc_free[i % C::SR], i / C::SR - 1);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sc_free[i % C::SR]);
+                    }
+                }
+                tiles += nall;
+            };
             if (u.state == 2) {
                 if (warp < 4) chunk_refuse<QT, D>(p, u, r, 128);
                 leave();
@@ -408,7 +424,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             const int tt = t * p.tile_tokens;              // first token of the tile in the unit
             const int cnt = min(u.n - tt, p.tile_tokens);  // its tokens
             if (cnt <= 0) {
-                tiles += nall;
+                pass(0);
                 leave();
                 continue;
             }
@@ -483,7 +499,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             for (int j = 0; j < nt; ++j) {
                 const int k0 = (kt0 + j) * CU_ROWS;  // first key
                 const bool masked = k0 + CU_ROWS > all_see;
-                const float* scales = s_scale + (tiles + j) % C::SR * 32;
+                const float* scales = s_scale + (tiles + j) % std::max(C::SR, 1) * 32;
                 lost = __any_sync(0xffffffffu, !wait(&s_full[t], ns++)) != 0;
                 if (lost) break;
                 tc_fence_after();
@@ -730,11 +746,14 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[t]);
+                if (lane == 0) {
+                    mbar_arrive(&p_full[t]);
+                    if constexpr (SRC == SRC_I8) mbar_arrive(&sc_free[(tiles + j) % C::SR]);
+                }
                 ++np;
             }
             if (lost) break;
-            tiles += nall;
+            pass(nt);
             settled();
             const volatile RingUnit& V = R;
             const bool bad = V.bad != 0, odd = V.odd != 0;
@@ -943,7 +962,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                         const float ks = ok ? __ldg(p.k_scale + (long long)id * p.Hkv + u.kvh) : 0.f;
                         const float vs = ok ? __ldg(p.v_scale + (long long)id * p.Hkv + u.kvh) : 0.f;
                         if (item >= RAWS) wait(&rk_empty[st], item / RAWS - 1);
-                        // (the slot's readers are done: fewer than SR key tiles are on their way)
+                        if (item >= C::SR) wait(&sc_free[item % C::SR], item / C::SR - 1);
                         const float vm = warp_max(vs <= 3.402823466e38f ? vs : 0.f);
                         if (lane < 16) {
                             s_scale[item % C::SR * 32 + lane] = ks;

@@ -263,6 +263,31 @@ def test_results_do_not_depend_on_what_ran_before(qt, kv, H, Hkv):
         assert torch.equal(run(), first)
 
 
+@pytest.mark.parametrize("qt", [F16, F32])
+@pytest.mark.parametrize("H,Hkv,D", [(33, 11, 64), (20, 4, 64), (33, 11, 128)])
+@pytest.mark.parametrize("new,ctx", [([181, 1], [9591, 133]), ([250, 1, 1, 1], [9244, 100, 133, 250]),
+                                     ([84] + [1] * 40, [1000] + [140] * 40)])
+def test_scales_stay_until_the_slower_query_tile_has_used_them(qt, H, Hkv, D, new, ctx):
+    # Units of one token have rows in one of the two query tiles only; the other one may still be in the unit before.
+    for seed in range(6):
+        c = make_cache(new, ctx, Hkv, D, 128, I8, seed)
+        q = make_q(sum(new), H, D, qt, seed + 1)
+        a = ops.PagedPrefill()
+
+        def run():
+            return a.chunk(q, c["k"], c["v"], c["table"], ints(c["total"]), starts(new), max_new=max(new),
+                           max_len=max(c["total"]), k_scale=c["ks"], v_scale=c["vs"], kernel=kvb.Kernel.umma)
+
+        first = run()
+        for _ in range(30):
+            assert torch.equal(run(), first)
+        at = 0
+        for b, n in enumerate(new):
+            want = attention64(q[at:at + n], rows_of(c, "k", b), rows_of(c, "v", b), ctx[b])
+            assert (first[at:at + n].double() - want).abs().max().item() <= tolerance(qt), (seed, b)
+            at += n
+
+
 @pytest.mark.parametrize("kv", [F16, I8])
 def test_pools_past_32_bits(kv):
     """Pages whose first value lies more than 2^31 elements into the pool (and 2^32 bytes)."""
