@@ -29,8 +29,9 @@
 // the exponentials as many, and under load the 1 kW power cap lowers the clock, so that the cap on sustained
 // library products (1375 of 1653 TFLOP/s) is the mark. A prompt of 8192 tokens (32 heads over 8, 0.55 TFLOP
 // that count): 445 us, 1240 TFLOP/s; 2048 tokens on a 32 k context: 920 us, 1160 TFLOP/s; 512 fp32 queries on
-// 32 k of int8 pages: 609 us, 900 TFLOP/s of the products with split operands. Few tokens on long contexts are
-// bound by memory and by the loads in flight (8 ragged chunks, 311 MB: 75 us, 4.1 TB/s) and, at the smallest, by
+// 32 k of int8 pages: 601 us, 910 TFLOP/s of the products with split operands (fp16 queries: 460 us; fp16
+// pages: 250 us. Converting the tiles and their scales are more code than the instruction cache holds beside
+// the rest). Few tokens on long contexts are bound by memory and by the loads in flight (8 ragged chunks, 311 MB: 75 us, 4.1 TB/s) and, at the smallest, by
 // the start, first loads and the join (4 x 3-8 tokens on 4 k, 57 MB: 28 us).
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -103,8 +104,8 @@ struct CCfg {
     static constexpr int RAW = CU_ROWS * D;                 // one int8 tile
     static constexpr int BUDGET = 227 * 1024 - 1024 - 2048;  // alignment, small arrays
     // Stages of K and of V: int8 tiles as loaded, fp16 tiles. (int8: few enough that the scales of SR key
-    // tiles cover those on their way.)
-    static constexpr int RAWS = SRC != SRC_I8 ? 0 : QF32 && D == 128 ? 1 : 2;
+    // tiles cover those on their way; at head dim 128 a second fp16 K tile is worth more than a second raw one.)
+    static constexpr int RAWS = SRC != SRC_I8 ? 0 : D == 128 ? 1 : 2;
     static constexpr int FIT = (BUDGET - 2 * QTILE - 2 * RAWS * RAW) / ITEM;
     static constexpr int MOST = SRC == SRC_I8 ? 6 : CU_CLEAN;
     static constexpr int STAGES = FIT > MOST ? MOST : FIT;
@@ -653,15 +654,18 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&s_free[t % C::SBUFS]);
                     settle_outputs();
-                    if constexpr (SRC == SRC_I8) {
-#pragma unroll
-                        for (int c = 0; c < CU_ROWS; c += 8) {
-                            const float ks = scales[c >> lp];  // (pages of 128 tokens or more: one)
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) s[c + i] = __float_as_uint(__uint_as_float(s[c + i]) * ks);
-                        }
-                    }
+                    // int8: the scale of a key's page is in the factor of its score, but for a masked tile's, whose
+                    // scores have it before -inf takes their places.
+                    auto factor = [&](int c) { return SRC == SRC_I8 && !masked ? f * scales[c >> lp] : f; };
                     if (masked) {
+                        if constexpr (SRC == SRC_I8) {
+#pragma unroll
+                            for (int c = 0; c < CU_ROWS; c += 8) {
+                                const float ks = scales[c >> lp];  // (pages of 128 tokens or more: one)
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) s[c + i] = __float_as_uint(__uint_as_float(s[c + i]) * ks);
+                            }
+                        }
                         const int lim = limit - k0;
 #pragma unroll
                         for (int c0 = 0; c0 < CU_ROWS; c0 += 32) {
@@ -676,14 +680,19 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     // The probabilities to tensor memory; their sum.
                     auto probabilities = [&]() {
                         const float base = ref == -INFINITY ? 0.f : -ref;
-                        const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
+                        const uint64_t b2 = pack2(base, base);
+                        uint64_t f2 = pack2(f, f), v2 = 0;
                         uint64_t l0 = 0, l1 = 0;
 #pragma unroll
                         for (int c0 = 0; c0 < CU_ROWS; c0 += 32) {
                             uint32_t pr[16];
-                            float vs = 0.f;
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
+                                if (SRC == SRC_I8 && i % 8 == 0) {  // pages of 8 tokens at least
+                                    const float fk = factor(c0 + i), vs = scales[16 + ((c0 + i) >> lp)] * vexp;
+                                    f2 = pack2(fk, fk);
+                                    v2 = pack2(vs, vs);
+                                }
                                 const uint64_t x =
                                     fma2(pack2(__uint_as_float(s[c0 + i]), __uint_as_float(s[c0 + i + 1])), f2, b2);
                                 float a, b;
@@ -696,16 +705,15 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                                 }
                                 if (i & 2) l1 = add2(l1, pack2(a, b));
                                 else l0 = add2(l0, pack2(a, b));
-                                if constexpr (SRC == SRC_I8) {
-                                    if (i % 8 == 0) vs = scales[16 + ((c0 + i) >> lp)] * vexp;  // pages of 8 tokens at least
-                                    a *= vs;
-                                    b *= vs;
-                                    if (masked) {  // the scale of a page that this row does not see may be anything
-                                        if (k0 + c0 + i >= limit) a = 0.f;
-                                        if (k0 + c0 + i + 1 >= limit) b = 0.f;
-                                    }
-                                }
+                                if constexpr (SRC == SRC_I8) unpack2(mul2(pack2(a, b), v2), a, b);
                                 pr[i / 2] = h2_as_u32(__floats2half2_rn(a, b));
+                            }
+                            if (SRC == SRC_I8 && masked) {  // the scale of a page that this row does not see may be anything
+                                const int n = limit - k0 - c0;
+                                const uint32_t sees = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
+#pragma unroll
+                                for (int i = 0; i < 16; ++i)
+                                    pr[i] &= (sees >> 2 * i & 1u ? 0xffffu : 0u) | (sees >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
                             }
                             tc_st16(tp + c0 / 2, pr);
                         }
@@ -724,10 +732,11 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                             float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
                             for (int i = 0; i < CU_ROWS; i += 4) {
-                                m0 = max3_nan(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                                m1 = max3_nan(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+                                const float fk = SRC == SRC_I8 ? factor(i) : 1.f;
+                                m0 = max3_nan(m0, __uint_as_float(s[i]) * fk, __uint_as_float(s[i + 1]) * fk);
+                                m1 = max3_nan(m1, __uint_as_float(s[i + 2]) * fk, __uint_as_float(s[i + 3]) * fk);
                             }
-                            top = fmaxf_nan(m0, m1) * f - CU_SHIFT;
+                            top = fmaxf_nan(m0, m1) * (SRC == SRC_I8 ? 1.f : f) - CU_SHIFT;
                             float scale = 1.f;
                             if (top > ref) {
                                 scale = ref == -INFINITY ? 0.f : ex2(ref - top);
@@ -1160,24 +1169,28 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                         const uint32_t rs = item % RR, st = item % N;
                         wait((is_v ? rv_full : rk_full) + rs, item / RR);
                         if (item >= N) wait((is_v ? v_empty : k_empty) + st, item / N - 1);
-                        const uint4* src = reinterpret_cast<const uint4*>(smem + C::RAW_OFF + ((is_v ? RAWS : 0) + rs) * C::RAW);
+                        const uint4* src = reinterpret_cast<const uint4*>(smem + C::RAW_OFF + ((is_v ? RAWS : 0) + rs) * C::RAW) + hh;
                         uint8_t* dst = smem + C::KV_OFF + ((is_v ? NK : 0) + st) * C::ITEM;
-#pragma unroll 4
-                        for (int i = hh; i < CU_ROWS * CH; i += 64) {
-                            const uint4 x = src[i];
-                            const int row = i / CH, c = i % CH;
-                            const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
-                            uint4 y[2];
-                            y[0] = make_uint4(i8pair_to_h2(w[0], SEL_B01), i8pair_to_h2(w[0], SEL_B23),
-                                              i8pair_to_h2(w[1], SEL_B01), i8pair_to_h2(w[1], SEL_B23));
-                            y[1] = make_uint4(i8pair_to_h2(w[2], SEL_B01), i8pair_to_h2(w[2], SEL_B23),
-                                              i8pair_to_h2(w[3], SEL_B01), i8pair_to_h2(w[3], SEL_B23));
-                            // lanes of the second slice store their halves in the other order: no bank twice
-                            uint8_t* slice = dst + (c / 4) * CU_SUB;
-                            const int flip = (c / 4) & 1;
-                            const uint32_t o0 = swz_off(row, (c % 4) * 32), o1 = swz_off(row, (c % 4) * 32 + 16);
-                            *reinterpret_cast<uint4*>(slice + (flip ? o1 : o0)) = flip ? y[1] : y[0];
-                            *reinterpret_cast<uint4*>(slice + (flip ? o0 : o1)) = flip ? y[0] : y[1];
+                        // A thread's pieces lie STEP rows apart, a multiple of 8, so their place in the swizzle is
+                        // the same. Lanes of the second slice take their halves in the other order: no bank twice.
+                        // Not unrolled: beside the softmax loop the instruction cache is what limits (512 queries
+                        // after 32 k int8 tokens, fp16 queries: 471 us, 8 pieces at a time 510 us).
+                        constexpr int STEP = 64 / CH;
+                        const int row = hh / CH, piece = hh % CH, flip = (piece / 4) & 1;
+                        uint8_t* slice = dst + (piece / 4) * CU_SUB;
+                        uint8_t* d0 = slice + swz_off(row, (piece % 4) * 32 + 16 * flip);
+                        uint8_t* d1 = slice + swz_off(row, (piece % 4) * 32 + 16 * (flip ^ 1));
+#pragma unroll 1
+                        for (int k = 0; k < CU_ROWS; k += STEP) {
+                            const uint4 x = src[k * CH];
+                            const uint32_t a = (flip ? x.z : x.x) ^ 0x80808080u, b = (flip ? x.w : x.y) ^ 0x80808080u;
+                            const uint32_t c = (flip ? x.x : x.z) ^ 0x80808080u, d = (flip ? x.y : x.w) ^ 0x80808080u;
+                            *reinterpret_cast<uint4*>(d0 + k * 128) =
+                                make_uint4(i8pair_to_h2(a, SEL_B01), i8pair_to_h2(a, SEL_B23), i8pair_to_h2(b, SEL_B01),
+                                           i8pair_to_h2(b, SEL_B23));
+                            *reinterpret_cast<uint4*>(d1 + k * 128) =
+                                make_uint4(i8pair_to_h2(c, SEL_B01), i8pair_to_h2(c, SEL_B23), i8pair_to_h2(d, SEL_B01),
+                                           i8pair_to_h2(d, SEL_B23));
                         }
                         fence_proxy_async_smem();
                         __syncwarp();
