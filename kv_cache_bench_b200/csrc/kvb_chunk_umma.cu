@@ -495,6 +495,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * scale);
                     tc_st16(to + c, o);
                 }
+                tc_wait_st();  // a second call for the same key tile loads what this one stored
             };
             bool lost = false;
             for (int j = 0; j < nt; ++j) {
@@ -583,6 +584,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                         bool raise = j == 0 && c0 == 0;
                         for (;;) {
                             if (raise) {
+                                tc_wait_st();  // the tile's probabilities so far are loaded again below
                                 float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
                                 for (int i = 0; i < 32; i += 4) {
@@ -729,6 +731,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     bool raise = j == 0;
                     for (;;) {
                         if (raise) {
+                            tc_wait_st();  // the probabilities stored so far are stored again
                             float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
                             for (int i = 0; i < CU_ROWS; i += 4) {

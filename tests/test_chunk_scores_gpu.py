@@ -1,0 +1,83 @@
+"""Attention of several new tokens per sequence where the scores are far apart: a row's running
+reference moves after its first key tile, inside a tile, past folded sums and between the pieces of a
+cut unit. Against 64 bits.
+
+All products of q and k are multiples of 2^-12 whose absolute sums stay below 2^12 (fp16 queries:
+2^-6 and 2^18), so every score is exact in fp32 in whatever order it is added up, and the tolerance is
+that of scores near 0.
+"""
+import math
+
+import pytest
+import torch
+
+import kv_cache_bench_b200 as kvb
+from kv_cache_bench_b200 import torch_ops as ops
+from tests.step_cases import F16, F32, I8, attention64, ints, make_cache, rows_of, starts, tolerance
+
+pytestmark = pytest.mark.gpu
+AUTO, SIMT = kvb.Kernel.auto, kvb.Kernel.simt
+
+
+def grid(shape, lo, hi, step, g):
+    return torch.randint(lo, hi + 1, shape, device="cuda", generator=g).float() * step
+
+
+def make_queries(T, H, D, qt, seed):
+    """First component 4, the others multiples of 1/8 up to 1; fp32 ones have bits that no fp16 holds."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = grid((T, H, D), -8, 8, 0.125, g)
+    q[:, :, 0] = 4.0
+    if qt is F32:
+        q += grid((T, H, D), -15, 15, 2.0 ** -9, g)
+    return q.to(qt)
+
+
+def set_keys(c, b, levels, D, kv, seed):
+    """Sequence b's keys: components that score about 0, and a first one that puts position j levels[j]
+    log2 units above that (against 4.0 in q)."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    L, page, Hkv = len(levels), c["page"], c["k"].shape[1]
+    first = torch.tensor(levels, dtype=torch.float64, device="cuda") * math.sqrt(D) / (4 * math.log2(math.e))
+    ids = c["table"][b, :-(-L // page)].long()
+    pos = torch.arange(L, device="cuda")
+    at = (ids[pos // page], slice(None), pos % page)
+    if kv is I8:  # scales of 8 and 4
+        scale = torch.where(torch.arange(len(ids), device="cuda") % 3 == 0, 4.0, 8.0)
+        if max(map(abs, levels)) * math.sqrt(D) / (4 * math.log2(math.e)) > 4 * 127:
+            scale[:] = 8.0
+        c["ks"][ids] = scale[:, None]
+        k = grid((L, Hkv, D), -1, 1, 1.0, g)
+        k[:, :, 0] = (first / scale[pos // page]).round().clamp(-127, 127).float()[:, None]
+    else:
+        k = grid((L, Hkv, D), -8, 8, 0.125, g)
+        k[:, :, 0] = (first * 8).round().float()[:, None] / 8
+    c["k"][at] = k.to(kv)
+
+
+def check(new, ctx, levels, H, Hkv, D, page, qt, kv, *, seed=1, kernel=AUTO):
+    """levels(position, tokens of the sequence): log2 units."""
+    c = make_cache(new, ctx, Hkv, D, page, kv, seed)
+    for b, total in enumerate(c["total"]):
+        set_keys(c, b, [levels(j, total) for j in range(total)], D, kv, seed + b)
+    q = make_queries(sum(new), H, D, qt, seed)
+    a = ops.PagedPrefill()
+    o = a.chunk(q, c["k"], c["v"], c["table"], ints(c["total"]), starts(new), max_new=max(new), max_len=max(c["total"]),
+                k_scale=c["ks"], v_scale=c["vs"], kernel=kernel)
+    assert a.error_flag() == 0
+    at = 0
+    for b, n in enumerate(new):
+        if n:
+            want = attention64(q[at:at + n], rows_of(c, "k", b), rows_of(c, "v", b), ctx[b])
+            err = (o[at:at + n].double() - want).abs().max().item()
+            assert err <= tolerance(qt), (b, n, ctx[b], err)
+        at += n
+
+
+@pytest.mark.parametrize("kv", [F16, I8])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("step", [10, 20, 50, 150, 400])
+def test_fp32_queries_reference_rises_inside_key_tiles(kv, D, step):
+    """Split probabilities that were written already follow the reference: every 32 keys it rises."""
+    check([70, 3], [500, 4000], lambda j, n: min(step * (j // 32), 450), 8, 2, D, 16, F32, kv)
+    check([70, 3], [500, 4000], lambda j, n: min(step * (j // 32 % 4), 450), 8, 2, D, 128, F32, kv)
