@@ -414,8 +414,8 @@ int kvb_paged_append(const kvb_append_args* args, void* stream);
  * max_new and max_len bound the new tokens and the total of any sequence (they size the grid). A
  * sequence that exceeds them, whose total is below its new tokens or above max_blocks * page_size (a
  * total of -1 from the plan, too), or that has rows outside [0, num_tokens), gets NaN rows and sets bit
- * 1; a live block id outside the pool NaN rows and bit 2. error_word is required: zero it once, read
- * it when convenient. The workspace needs no preparation and holds nothing between calls. At most 64
+ * 1; a live block id outside the pool makes the rows of the tokens that see its page NaN and sets bit 2.
+ * error_word is required: zero it once, read it when convenient. The workspace needs no preparation and holds nothing between calls. At most 64
  * query heads per KV head. q and the pools 16-byte aligned, q's stride whole 16 bytes; out and the
  * workspace 32-byte aligned. */
 typedef struct kvb_chunk_args {

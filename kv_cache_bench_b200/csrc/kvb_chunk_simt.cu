@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(SM_THREADS) chunk_simt_kernel(const __grid_con
     float* sp = reinterpret_cast<float*>(smem + C::P_OFF);
     __shared__ const KT* s_rows[2][SM_KEYS];
     __shared__ float s_scale[2][SM_KEYS];
-    __shared__ int s_bad, s_odd;
+    __shared__ int s_bad, s_odd;  // first position whose block id was refused; a masked value was not finite
     const int tid = threadIdx.x, rg = tid >> 3, cg = tid & 7;
     pdl_wait();
     pdl_trigger();
@@ -70,7 +70,10 @@ __global__ void __launch_bounds__(SM_THREADS) chunk_simt_kernel(const __grid_con
     }
     const int h0 = u.kvh * p.G;
     const int rows = u.n * p.G;  // <= SM_ROWS
-    if (tid == 0) s_bad = s_odd = 0;
+    if (tid == 0) {
+        s_bad = 0x7fffffff;
+        s_odd = 0;
+    }
     for (int i = tid; i < SM_ROWS * D4; i += SM_THREADS) {
         const int r = i / D4, c = i % D4;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -103,7 +106,7 @@ __global__ void __launch_bounds__(SM_THREADS) chunk_simt_kernel(const __grid_con
             if (k0 + j < u.keys) {
                 row = which ? chunk_row<KT>(p, u, p.v, p.v_stride, k0 + j, D)
                             : chunk_row<KT>(p, u, p.k, p.k_stride, k0 + j, D);
-                if (!row) s_bad = 1;
+                if (!row) atomicMin(&s_bad, k0 + j);
                 if (sizeof(KT) == 1 && row) {
                     const int id = __ldg(p.block_table + (size_t)u.b * p.max_blocks + (k0 + j) / p.page);
                     sc = __ldg((which ? p.v_scale : p.k_scale) + (long long)id * p.Hkv + u.kvh);
@@ -199,14 +202,16 @@ __global__ void __launch_bounds__(SM_THREADS) chunk_simt_kernel(const __grid_con
         }
     }
     __syncthreads();
-    const bool bad = s_bad, odd = s_odd;
-    if (bad && tid == 0) raise_error(p.error_flag, KVB_DEVERR_BLOCK);
+    const int bad_from = s_bad;
+    const bool odd = s_odd;
+    if (bad_from < u.keys && tid == 0) raise_error(p.error_flag, KVB_DEVERR_BLOCK);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int off = 1; off < 8; off <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
         const int r = rg + 16 * i;
         if (r >= rows) continue;
+        const bool bad = bad_from < limit[i];  // the rows that see it are NaN
         if (odd && !bad) {
             const int first = max(tiles.x * SM_KEYS, seen_by_all / SM_KEYS * SM_KEYS);
             for (int j = first; j < min(limit[i], tiles.y * SM_KEYS); ++j) {

@@ -147,7 +147,9 @@ struct RingUnit {
     int nt[2];      // key tiles of the two query tiles
     int slot;       // where its partial result goes; -1: the unit is whole
     int odd;        // a seen value was not finite (set by the cleaning warps)
-    int bad;        // a block id was refused (set by the producer)
+    int bad;        // first position whose block id was refused (the producers' minimum): the rows that see it are
+                    // NaN. A query tile with fewer key tiles may read it while a later one's is set: no row of it
+                    // sees that position
 };
 static_assert(sizeof(RingUnit) <= 64, "ring entry");
 
@@ -768,8 +770,8 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             pass(nt);
             settled();
             const volatile RingUnit& V = R;
-            const bool bad = V.bad != 0, odd = V.odd != 0;
-            if (bad && r == 0) raise_error(p.error_flag, KVB_DEVERR_BLOCK);
+            const bool bad = V.bad < limit, odd = V.odd != 0;
+            if (__any_sync(0xffffffffu, bad) && lane == 0) raise_error(p.error_flag, KVB_DEVERR_BLOCK);
             float inv = bad ? __int_as_float(0x7fc00000) : slot >= 0 && l == 0.f ? 0.f : 1.f / l;
             const size_t row = (size_t)qrow * p.H + h;
             const size_t at = ((size_t)slot * 2 + t) * CU_ROWS + r;
@@ -842,7 +844,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             const int k = tile * CU_ROWS + lane * bt;
             const bool wanted = SRC != SRC_PACKED && lane * bt < CU_ROWS && k < u.keys;
             const bool ok = wanted && id >= 0 && id < p.num_blocks;
-            if (__any_sync(0xffffffffu, wanted && !ok) && lane == 0) reinterpret_cast<volatile RingUnit&>(R).bad = 1;
+            if (wanted && !ok) atomicMin(&R.bad, k);
             const uint32_t boxes = SRC == SRC_PACKED ? 1 : __popc(__ballot_sync(0xffffffffu, ok));
             const uint32_t bytes = SRC == SRC_I8 ? uint32_t(bt) * D : uint32_t(bt) * 128 * NSUB;  // of a box
             const bool off = *s_abort != 0;
@@ -888,7 +890,8 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     R.nt[0] = nt0;
                     R.nt[1] = nt1;
                     R.slot = slot;
-                    R.odd = R.bad = 0;
+                    R.odd = 0;
+                    R.bad = 0x7fffffff;
                     mbar_arrive(&r_full[published % CU_RING]);
                 }
                 ++published;
