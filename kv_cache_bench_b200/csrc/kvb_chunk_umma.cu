@@ -170,6 +170,11 @@ __device__ __forceinline__ float fmaxf_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
+__device__ __forceinline__ float fminf_nan(float a, float b) {
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
 
 // Two fp32 operations per instruction.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
@@ -198,11 +203,12 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 
 // 2^x of a pair on the FMA pipe: x = n + r with n the nearest integer and r in [-1/2, 1/2], 2^r by its
 // minimax polynomial of degree 4 (fitted to the relative error, 2.6e-6, far below the fp16 rounding that
-// follows), times 2^n. x + 1.5 * 2^23 + 127 holds n + 127, 2^n's exponent, in its low bits. x is taken as at
-// least -126; NaN stays NaN.
+// follows), times 2^n. x + 1.5 * 2^23 + 127 holds n + 127, 2^n's exponent, in its low bits. x is taken into
+// [-127, 127], where that is 0 (a factor of 0) to 254: with a reference that a key tile has left far behind x has
+// no bound, and 2^127 makes the sum raise the reference as infinity would. NaN stays NaN.
 __device__ __forceinline__ void exp2_poly2(uint64_t x, float& a, float& b) {
     unpack2(x, a, b);
-    x = pack2(fmaxf_nan(a, -126.f), fmaxf_nan(b, -126.f));
+    x = pack2(fminf_nan(fmaxf_nan(a, -127.f), 127.f), fminf_nan(fmaxf_nan(b, -127.f), 127.f));
     const uint64_t magic = pack2(12583039.f, 12583039.f), minus = pack2(-12583039.f, -12583039.f);
     const uint64_t n = add2(x, magic);
     const uint64_t r = fma2(add2(n, minus), pack2(-1.f, -1.f), x);

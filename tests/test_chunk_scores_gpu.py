@@ -81,3 +81,57 @@ def test_fp32_queries_reference_rises_inside_key_tiles(kv, D, step):
     """Split probabilities that were written already follow the reference: every 32 keys it rises."""
     check([70, 3], [500, 4000], lambda j, n: min(step * (j // 32), 450), 8, 2, D, 16, F32, kv)
     check([70, 3], [500, 4000], lambda j, n: min(step * (j // 32 % 4), 450), 8, 2, D, 128, F32, kv)
+
+
+ONE_IN_32 = list(range(32))
+
+
+@pytest.mark.parametrize("kind", ["pages", "int8 pages", "prompt"])
+@pytest.mark.parametrize("up", [126, 128.2, 130, 200, 300, 400, 500])
+def test_one_key_far_above_the_first_tile_counts_wherever_it_lies(kind, up):
+    """Head dim 64: part of the exponentials are a polynomial, by the key's place among 32. A batch of 32
+    sequences, the key of sequence b at position 128 + b, `up` log2 units above the others."""
+    H, Hkv, D, n = 4, 2, 64, 12
+    new, ctx = [n] * 32, [200] * 32
+    kv = I8 if kind == "int8 pages" else F16
+    if kind != "prompt":
+        c = make_cache(new, ctx, Hkv, D, 64, kv, 5)
+        for b in ONE_IN_32:
+            set_keys(c, b, [up if j == 128 + b else 0.0 for j in range(212)], D, kv, b)
+        q = make_queries(n * 32, H, D, F16, 6)
+        a = ops.PagedPrefill()
+        o = a.chunk(q, c["k"], c["v"], c["table"], ints(c["total"]), starts(new), max_new=n, max_len=212,
+                    k_scale=c["ks"], v_scale=c["vs"])
+        for b in ONE_IN_32:
+            want = attention64(q[n * b:n * (b + 1)], rows_of(c, "k", b), rows_of(c, "v", b), 200)
+            assert (o[n * b:n * (b + 1)].double() - want).abs().max().item() <= tolerance(F16), b
+        return
+    c = make_cache([212] * 32, [0] * 32, Hkv, D, 64, F16, 5)  # the same rows, packed
+    for b in ONE_IN_32:
+        set_keys(c, b, [up if j == 128 + b else 0.0 for j in range(212)], D, F16, b)
+    k, v = (torch.cat([rows_of(c, x, b) for b in ONE_IN_32]) for x in "kv")
+    q = make_queries(212 * 32, H, D, F16, 6)
+    o = ops.PagedPrefill().prompt(q, k.half(), v.half(), starts([212] * 32), max_len=212)
+    for b in ONE_IN_32:
+        x = slice(212 * b, 212 * (b + 1))
+        assert (o[x].double() - attention64(q[x], k[x], v[x], 0)).abs().max().item() <= tolerance(F16), b
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kv", [F16, I8])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_an_infinite_or_nan_score_makes_the_row_nan(D, kv, bad):
+    """... in a later key tile, at every place among 32."""
+    new, ctx = [3] * 32, [300] * 32
+    c = make_cache(new, ctx, 1, D, 16, kv, 7)
+    for b in ONE_IN_32:
+        p = 128 + b
+        if kv is I8:
+            c["k"][c["table"][b, p // 16].long(), 0, :, :] = 1
+            c["ks"][c["table"][b, p // 16].long(), 0] = bad
+        else:
+            c["k"][c["table"][b, p // 16].long(), 0, p % 16, 0] = bad
+    q = make_queries(96, 2, D, F16, 6).abs()
+    o = ops.PagedPrefill().chunk(q, c["k"], c["v"], c["table"], ints(c["total"]), starts(new), max_new=3, max_len=303,
+                                 k_scale=c["ks"], v_scale=c["vs"])
+    assert o.isnan().all()
