@@ -806,7 +806,9 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     }
                 }
                 if (SRC != SRC_I8 && odd && !bad && live) {
-                    const int first = max(kt0, all_see / CU_ROWS) * CU_ROWS;
+                    // (the tiles are cleaned from the first one that some row of the unit, not of this query
+                    // tile, does not see in full)
+                    const int first = max(kt0, (u.pos0 + 1) / CU_ROWS) * CU_ROWS;
                     for (int k = first; k < min(limit, (kt0 + nt) * CU_ROWS); ++k) {
                         const __half* v = chunk_row<__half>(p, u, p.v, p.v_stride, k, D) + c;
 #pragma unroll

@@ -1,0 +1,51 @@
+"""Non-finite values and keys in attention of several new tokens per sequence, in units of one and of two
+query tiles, whole and cut: they reach the tokens that see them, and no other."""
+import pytest
+import torch
+
+import kv_cache_bench_b200 as kvb
+from kv_cache_bench_b200 import torch_ops as ops
+from tests.step_cases import F16, F32, attention64, ints, make_cache, make_q, rows_of, starts, tolerance
+
+pytestmark = pytest.mark.gpu
+AUTO, SIMT = kvb.Kernel.auto, kvb.Kernel.simt
+
+
+def same(o, want, qt):
+    fine = torch.isfinite(want)
+    assert torch.equal(fine, torch.isfinite(o))
+    assert torch.where(fine, o.double() - want, 0.0).abs().max().item() <= tolerance(qt)
+
+
+# Query heads per KV head, new tokens, tokens before them, and where the values lie: before the unit's second
+# query tile, with the tiles' first masked key tiles the same and different ones.
+PLACES = [(1, 256, 0, 5), (1, 256, 0, 127), (1, 256, 0, 128), (1, 600, 0, 300), (1, 200, 60, 70), (4, 64, 100, 110),
+          (4, 40, 100, 127), (4, 64, 100, 128), (4, 64, 3000, 3010), (2, 500, 2000, 2100), (7, 36, 120, 122),
+          (64, 4, 126, 127)]
+
+
+@pytest.mark.parametrize("kernel", [AUTO, SIMT])
+@pytest.mark.parametrize("qt,kv", [(F16, F16), (F32, F16), (F32, F32)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G,n,ctx,at", PLACES)
+def test_values_of_the_new_tokens(kernel, qt, kv, D, G, n, ctx, at):
+    c = make_cache([n], [ctx], 2, D, 16, kv, seed=5)
+    q = make_q(n, 2 * G, D, qt, 6)
+    for d, (p, x) in enumerate(((at, float("inf")), (at + 1, float("nan")), (at + 2, -float("inf")))):
+        if p < n + ctx:
+            c["v"][c["table"][0, p // 16].long(), 0, p % 16, 3 + d] = x
+    o = ops.PagedPrefill().chunk(q, c["k"], c["v"], c["table"], ints(c["total"]), starts([n]), max_new=n, max_len=n + ctx,
+                                 kernel=kernel)
+    same(o, attention64(q, rows_of(c, "k", 0), rows_of(c, "v", 0), ctx), qt)
+
+
+@pytest.mark.parametrize("kernel", [AUTO, SIMT])
+@pytest.mark.parametrize("dt", [F16, F32])
+@pytest.mark.parametrize("G,n,at", [(G, n, at) for G, n, ctx, at in PLACES if ctx == 0] + [(4, 3000, 1030)])
+def test_values_of_a_prompt(kernel, dt, G, n, at):
+    q, k, v = (make_q(n + 9, h, 128, dt, h) for h in (2 * G, 2, 3))
+    v = v[:, :2].contiguous()
+    v[at, 0, 3], v[at + 1, 0, 4], v[at + 2, 0, 5] = float("inf"), float("nan"), -float("inf")
+    o = ops.PagedPrefill().prompt(q, k, v, starts([n, 9]), max_len=n, kernel=kernel)
+    for x in (slice(0, n), slice(n, n + 9)):
+        same(o[x], attention64(q[x], k[x].double(), v[x].double(), 0), dt)
