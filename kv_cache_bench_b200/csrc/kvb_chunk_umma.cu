@@ -479,7 +479,9 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 }
             }
             float ref = -INFINITY;  // probabilities are 2^(f s - ref)
-            const float most = live ? CU_MOST : INFINITY;  // rows of no token hold anything: they move no reference
+            // What a key tile's probabilities may sum to before the reference moves: anything at all until there is
+            // one (every score so far was -inf). Rows of no token hold anything: they move no reference.
+            float most = live ? -1.f : INFINITY;
             float l = 0.f;
             float vexp = 0.f;       // int8: 2^-e, probabilities times the value scales times this; 0: not set
             float older = 1.f;      // what the folded sum has to be scaled by
@@ -605,6 +607,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                                 if (up > ref) {
                                     scale = ref == -INFINITY ? 0.f : ex2(ref - up);
                                     ref = up;
+                                    if (live) most = CU_MOST;
                                     l *= scale;
                                     sum *= scale;
                                 }
@@ -732,9 +735,8 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                         return a + b;
                     };
                     // With the reference so far first. No probability is above their sum, so a sum in bounds needs
-                    // no maximum (a NaN makes the row NaN as it is). Otherwise, and at the first key tile, the
-                    // reference rises to the highest score, O and l follow, and the probabilities are computed
-                    // with that. (One copy of their code: the instruction cache holds little more than the loop.)
+                    // no maximum (a NaN makes the row NaN as it is). Otherwise, and until there is a reference, it
+                    // rises to the highest score, O and l follow, and the probabilities are computed with that. (One copy of their code: the instruction cache holds little more than the loop.)
                     float top = 0.f;
                     bool raise = j == 0;
                     for (;;) {
@@ -752,6 +754,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                             if (top > ref) {
                                 scale = ref == -INFINITY ? 0.f : ex2(ref - top);
                                 ref = top;
+                                if (live) most = CU_MOST;
                                 l *= scale;
                             }
                             if (j > 0) rescale(scale);

@@ -135,3 +135,50 @@ def test_an_infinite_or_nan_score_makes_the_row_nan(D, kv, bad):
     o = ops.PagedPrefill().chunk(q, c["k"], c["v"], c["table"], ints(c["total"]), starts(new), max_new=3, max_len=303,
                                  k_scale=c["ks"], v_scale=c["vs"])
     assert o.isnan().all()
+
+
+def lowest(c, b, positions, kv):
+    """Keys whose score is -inf for queries without a negative or zero component."""
+    page = c["page"]
+    for p in positions:
+        blk = c["table"][b, p // page].long()
+        if kv is I8:  # whole pages
+            c["k"][blk], c["ks"][blk] = -1, float("inf")
+        else:
+            c["k"][blk, :, p % page, :] = -1.0
+            c["k"][blk, :, p % page, 0] = -float("inf")
+
+
+@pytest.mark.parametrize("qt,kv", [(F16, F16), (F16, I8), (F32, I8), (F32, F32)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("level", [0, -12, -20, -30, -80, -200])
+@pytest.mark.parametrize("new,ctx,dead", [([5], [400], range(128)), ([130], [256], range(160)), ([3], [400], range(48)),
+                                          ([3], [6000], range(2048)), ([3], [6000], range(1024, 4096))])
+def test_a_first_key_tile_of_infinitely_low_scores(qt, kv, D, level, new, ctx, dead):
+    """The row's reference is set by the first score that is finite, however low it lies."""
+    c = make_cache(new, ctx, 2, D, 16, kv, 3)
+    set_keys(c, 0, [float(level)] * c["total"][0], D, kv, 4)
+    lowest(c, 0, dead, kv)
+    q = make_queries(sum(new), 8, D, qt, 5).abs().clamp(min=0.125)
+    a = ops.PagedPrefill()
+    for kernel in (AUTO, SIMT):
+        o = a.chunk(q, c["k"], c["v"], c["table"], ints(c["total"]), starts(new), max_new=max(new), max_len=c["total"][0],
+                    k_scale=c["ks"], v_scale=c["vs"], kernel=kernel)
+        want = attention64(q, rows_of(c, "k", 0), rows_of(c, "v", 0), ctx[0])
+        assert (o.double() - want).abs().max().item() <= tolerance(qt)
+
+
+@pytest.mark.parametrize("dt", [F16, F32])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_prompt_whose_first_keys_score_infinitely_low(dt, D):
+    """Tokens that see no other key have no softmax (NaN); the others are the mean over the rest."""
+    c = make_cache([500], [0], 2, D, 16, F32, 3)
+    set_keys(c, 0, [-40.0] * 500, D, F32, 4)
+    lowest(c, 0, range(140), F32)
+    k, v = (rows_of(c, x, 0).to(dt) for x in "kv")
+    q = make_queries(500, 8, D, dt, 5).abs().clamp(min=0.125)
+    for kernel in (AUTO, SIMT):
+        o = ops.PagedPrefill().prompt(q, k, v, starts([500]), max_len=500, kernel=kernel)
+        want = attention64(q, k.double(), v.double(), 0)
+        assert o[:140].isnan().all() and want[:140].isnan().all()
+        assert (o[140:].double() - want[140:]).abs().max().item() <= tolerance(dt)
