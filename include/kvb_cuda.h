@@ -410,7 +410,9 @@ int kvb_paged_append(const kvb_append_args* args, void* stream);
  * sequence is its decode step. q and out are both fp32 (fp32-level results) or both fp16 (the
  * probabilities are rounded to fp16 for the value product; sums and maxima are fp32).
  * Values behind a sequence's last token are never used, whatever bits they hold; a non-finite key or
- * value reaches the tokens that see it and no other.
+ * value reaches the tokens that see it and no other. A key that scores -inf has no weight, one that
+ * scores +inf or NaN makes the token's row NaN; an infinite value may arrive as NaN (its probability is
+ * rounded to fp16, with fp32 queries held in two fp16 parts, and infinity times 0 is NaN).
  * max_new and max_len bound the new tokens and the total of any sequence (they size the grid). A
  * sequence that exceeds them, whose total is below its new tokens or above max_blocks * page_size (a
  * total of -1 from the plan, too), or that has rows outside [0, num_tokens), gets NaN rows and sets bit

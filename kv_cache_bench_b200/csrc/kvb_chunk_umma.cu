@@ -507,6 +507,28 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 }
                 tc_wait_st();  // a second call for the same key tile loads what this one stored
             };
+            // fp32 queries on fp16 pages: the scores that are NaN among 32 of a key tile once more, in fp32 (on keys
+            // with an infinite component, so that their scale does not matter: -inf, +inf or NaN).
+            auto rescore = [&](int k0, int c0) {
+                const float* qr = static_cast<const float*>(p.q) + qrow * p.q_stride + (long long)h * D;
+#pragma unroll 1
+                for (int c = c0; c < c0 + 32; ++c) {
+                    uint32_t x = tc_ld1(ts + c);
+                    tc_wait_ld();
+                    pin<1>(&x);
+                    const bool odd = __uint_as_float(x) != __uint_as_float(x) && k0 + c < limit;
+                    const __half* kr = odd ? chunk_row<__half>(p, u, p.k, p.k_stride, k0 + c, D) : nullptr;
+                    if (kr) {
+                        float y = 0.f;
+#pragma unroll 1
+                        for (int i = 0; i < D; ++i) y = fmaf(qr[i], __half2float(kr[i]), y);
+                        x = __float_as_uint(y);
+                    }
+                    __syncwarp();
+                    tc_st1(ts + c, x);
+                }
+                tc_wait_st();
+            };
             bool lost = false;
             for (int j = 0; j < nt; ++j) {
                 const int k0 = (kt0 + j) * CU_ROWS;  // first key
@@ -572,86 +594,96 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
 #pragma unroll 1
                     for (int c0 = 0; c0 < CU_ROWS; c0 += 32) {
                         uint32_t s[32], pr[32];
-                        tc_ld32(ts + c0, s);
-                        tc_wait_ld();
-                        pin<32>(s);
-                        if constexpr (SRC == SRC_I8) {
-#pragma unroll
-                            for (int c = 0; c < 32; c += 8) {
-                                const float ks = scales[(c0 + c) >> lp];
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) s[c + i] = __float_as_uint(__uint_as_float(s[c + i]) * ks);
-                            }
-                        }
-                        const int lim = limit - k0 - c0;
-                        if (masked) {
-                            const uint32_t sees = lim >= 32 ? ~0u : lim <= 0 ? 0u : (1u << lim) - 1u;
-#pragma unroll
-                            for (int c = 0; c < 32; ++c)
-                                if (!(sees >> c & 1u)) s[c] = 0xff800000u;  // -inf
-                        }
-                        float part = 0.f, top = 0.f;
-                        bool raise = j == 0 && c0 == 0;
-                        for (;;) {
-                            if (raise) {
-                                tc_wait_st();  // the tile's probabilities so far are loaded again below
-                                float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-                                for (int i = 0; i < 32; i += 4) {
-                                    m0 = max3_nan(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                                    m1 = max3_nan(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
-                                }
-                                top = fmaxf_nan(m0, m1) * f;
-                                const float up = ceilf(top) - CU_SHIFT;
-                                float scale = 1.f;
-                                if (up > ref) {
-                                    scale = ref == -INFINITY ? 0.f : ex2(ref - up);
-                                    ref = up;
-                                    if (live) most = CU_MOST;
-                                    l *= scale;
-                                    sum *= scale;
-                                }
-                                if (j > 0) rescale(scale);
-                                const __half2 by = __float2half2_rn(scale);  // a power of two, or 0 when none is left
+                        float part, top;
 #pragma unroll 1
-                                for (int c = 0; c < c0; c += 16) {
-                                    uint32_t w[16];
-                                    tc_ld16(tp + c, w);
-                                    tc_wait_ld();
-                                    pin<16>(w);
+                        for (bool again = false;; again = true) {
+                            tc_ld32(ts + c0, s);
+                            tc_wait_ld();
+                            pin<32>(s);
+                            if constexpr (SRC == SRC_I8) {
 #pragma unroll
-                                    for (int i = 0; i < 16; ++i) w[i] = h2_as_u32(__hmul2(u32_as_h2(w[i]), by));
-                                    tc_st16(tp + c, w);
+                                for (int c = 0; c < 32; c += 8) {
+                                    const float ks = scales[(c0 + c) >> lp];
+#pragma unroll
+                                    for (int i = 0; i < 8; ++i) s[c + i] = __float_as_uint(__uint_as_float(s[c + i]) * ks);
                                 }
                             }
-                            const float base = ref == -INFINITY ? 0.f : -ref;
-                            const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
-                            uint64_t l0 = 0, l1 = 0;
-                            float vs = 0.f;
+                            const int lim = limit - k0 - c0;
+                            if (masked) {
+                                const uint32_t sees = lim >= 32 ? ~0u : lim <= 0 ? 0u : (1u << lim) - 1u;
 #pragma unroll
-                            for (int i = 0; i < 32; i += 2) {
-                                float a, b;
-                                unpack2(fma2(pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, b2), a, b);
-                                a = ex2(a);
-                                b = ex2(b);
-                                if (i & 2) l1 = add2(l1, pack2(a, b));
-                                else l0 = add2(l0, pack2(a, b));
-                                if constexpr (SRC == SRC_I8) {
-                                    if (i % 8 == 0) vs = scales[16 + ((c0 + i) >> lp)] * vexp;  // pages of 8 tokens at least
-                                    a *= vs;
-                                    b *= vs;
-                                    if (masked) {  // the scale of a page that this row does not see may be anything
-                                        if (i >= lim) a = 0.f;
-                                        if (i + 1 >= lim) b = 0.f;
+                                for (int c = 0; c < 32; ++c)
+                                    if (!(sees >> c & 1u)) s[c] = 0xff800000u;  // -inf
+                            }
+                            part = top = 0.f;
+                            bool raise = j == 0 && c0 == 0;
+                            for (;;) {
+                                if (raise) {
+                                    tc_wait_st();  // the tile's probabilities so far are loaded again below
+                                    float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+                                    for (int i = 0; i < 32; i += 4) {
+                                        m0 = max3_nan(m0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                                        m1 = max3_nan(m1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+                                    }
+                                    top = fmaxf_nan(m0, m1) * f;
+                                    const float up = ceilf(top) - CU_SHIFT;
+                                    float scale = 1.f;
+                                    if (up > ref) {
+                                        scale = ref == -INFINITY ? 0.f : ex2(ref - up);
+                                        ref = up;
+                                        if (live) most = CU_MOST;
+                                        l *= scale;
+                                        sum *= scale;
+                                    }
+                                    if (j > 0) rescale(scale);
+                                    const __half2 by = __float2half2_rn(scale);  // a power of two, or 0 when none is left
+#pragma unroll 1
+                                    for (int c = 0; c < c0; c += 16) {
+                                        uint32_t w[16];
+                                        tc_ld16(tp + c, w);
+                                        tc_wait_ld();
+                                        pin<16>(w);
+#pragma unroll
+                                        for (int i = 0; i < 16; ++i) w[i] = h2_as_u32(__hmul2(u32_as_h2(w[i]), by));
+                                        tc_st16(tp + c, w);
                                     }
                                 }
-                                split_hi_lo(a, b, pr[i / 2], pr[16 + i / 2]);
+                                const float base = ref == -INFINITY ? 0.f : -ref;
+                                const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
+                                uint64_t l0 = 0, l1 = 0;
+                                float vs = 0.f;
+#pragma unroll
+                                for (int i = 0; i < 32; i += 2) {
+                                    float a, b;
+                                    unpack2(fma2(pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, b2), a, b);
+                                    a = ex2(a);
+                                    b = ex2(b);
+                                    if (i & 2) l1 = add2(l1, pack2(a, b));
+                                    else l0 = add2(l0, pack2(a, b));
+                                    if constexpr (SRC == SRC_I8) {
+                                        if (i % 8 == 0) vs = scales[16 + ((c0 + i) >> lp)] * vexp;  // pages of 8 tokens at least
+                                        a *= vs;
+                                        b *= vs;
+                                        if (masked) {  // the scale of a page that this row does not see may be anything
+                                            if (i >= lim) a = 0.f;
+                                            if (i + 1 >= lim) b = 0.f;
+                                        }
+                                    }
+                                    split_hi_lo(a, b, pr[i / 2], pr[16 + i / 2]);
+                                }
+                                float a, b;
+                                unpack2(add2(l0, l1), a, b);
+                                part = a + b;
+                                if (raise || !__any_sync(0xffffffffu, part > most)) break;
+                                raise = true;
                             }
-                            float a, b;
-                            unpack2(add2(l0, l1), a, b);
-                            part = a + b;
-                            if (raise || !__any_sync(0xffffffffu, part > most)) break;
-                            raise = true;
+                            // A NaN that is the row's first may come from an infinite key and the two parts of a
+                            // query, of which one may be 0 or of the other sign.
+                            if (SRC != SRC_F16 || again ||
+                                !__any_sync(0xffffffffu, part != part && sum == sum && l == l))
+                                break;
+                            rescore(k0, c0);
                         }
                         tc_st32(tp + c0, pr);
                         sum += top < INFINITY ? part : __int_as_float(0x7fc00000);

@@ -49,3 +49,38 @@ def test_values_of_a_prompt(kernel, dt, G, n, at):
     o = ops.PagedPrefill().prompt(q, k, v, starts([n, 9]), max_len=n, kernel=kernel)
     for x in (slice(0, n), slice(n, n + 9)):
         same(o[x], attention64(q[x], k[x].double(), v[x].double(), 0), dt)
+
+
+@pytest.mark.parametrize("kernel", [AUTO, SIMT])
+@pytest.mark.parametrize("qt,kv", [(F16, F16), (F32, F16), (F32, F32)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G,n,ctx,at", [(4, 40, 100, [3]), (1, 300, 0, [0, 70, 200]), (4, 5, 3000, [10, 31, 32, 1500, 3001]),
+                                        (2, 200, 700, list(range(50, 600, 7))), (8, 3, 200, list(range(128)))])
+def test_infinite_keys(kernel, qt, kv, D, G, n, ctx, at):
+    """An infinite component of a key scores -inf (no weight) or +inf (NaN) by the query's sign, and NaN where that is
+    0 or another component is infinite the other way; queries too small for the fp16 parts of the row count too."""
+    c = make_cache([n], [ctx], 2, D, 16, kv, seed=5)
+    q = make_q(n, 2 * G, D, qt, 6)
+    q[:, :, 7] = -q[:, :, 7].abs() - 0.25
+    q[:, 1:, 9] = q[:, 1:, 9].abs() + 1e-3  # (head 0: any sign)
+    q[n // 2, 0, 9] = 0.0
+    if qt is F32:
+        q[1::3, :, 7] = -1e-9
+        q[n - 1, -1, 7] = -1e-30
+    for i, p in enumerate(at):
+        k = c["k"][c["table"][0, p // 16].long()]
+        k[0, p % 16, 7 if i % 2 == 0 else 9] = float("inf") if i % 2 == 0 else -float("inf")
+        k[1, p % 16, 7] = float("inf")
+        if i == 2:
+            k[1, p % 16, 9] = -float("inf")
+    a = ops.PagedPrefill()
+
+    def run():
+        return a.chunk(q, c["k"], c["v"], c["table"], ints(c["total"]), starts([n]), max_new=n, max_len=n + ctx,
+                       kernel=kernel)
+
+    o = run()
+    want = attention64(q, rows_of(c, "k", 0), rows_of(c, "v", 0), ctx)
+    assert want[:, 2 * G - 1].isfinite().any()
+    same(o, want, qt)
+    assert torch.equal(o.nan_to_num(7), run().nan_to_num(7))
