@@ -377,7 +377,9 @@ int kvb_step_plan(const kvb_step_plan_args* args, void* stream);
  *   KV head), with amax the largest |x| of the new rows in it, s = amax / 127 (fp32), or the page's
  *   scale so far where that is larger and the page held rows before; those rows are rounded again,
  *   rint(q * (s_old / s)), when the scale grew; new rows are clamp(rint(x / s), -127, 127), 0 for s = 0.
- *   Rows of a page from its first slot on in one append give what kvb_quantize_paged_i8 gives. A
+ *   A NaN or infinite row makes s NaN or infinite and the page's rows 0, and such a scale stays until the
+ *   page is begun anew (its first slot appended): the page reads as NaN, not as numbers.
+ *   Finite rows of a page from its first slot on in one append give what kvb_quantize_paged_i8 gives. A
  *   sequence with total_lens -1 is skipped; one whose total is below its new tokens or above
  *   max_blocks * page_size is skipped with bit 1; a block id outside the pool skips its page with bit
  *   2. A page may belong to one appending sequence only.

@@ -230,15 +230,23 @@ __device__ __forceinline__ float4 load4(const SRC* s) {
     }
 }
 
+// Larger of the two, NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
 __device__ __forceinline__ float amax4(float4 v) {
-    return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+    return max_nan(max_nan(fabsf(v.x), fabsf(v.y)), max_nan(fabsf(v.z), fabsf(v.w)));
 }
 
 // int8 pools. A run is the new tokens of one sequence that share a page, for one KV head of K or V, and TPR
 // threads (a warp, or the CTA for pages of 32 KB of fp32 and more) take it. The page's scale becomes
 // s = max(s_old, amax / 127) (s_old only if the page had rows before); rows that were there are rounded
 // again, rint(q * (s_old / s)), when the scale grew; new rows by the page quantizer's rule (kvb_quant.cuh). A
-// token starts a run if it is its sequence's first new one or the first of its page; each group looks for
+// NaN among the rows makes amax and s NaN (rows 0), and a scale that is not finite stays until the page is begun
+// anew, so that no value which is not finite turns into a number. A token starts a run if it is its sequence's first new one or the first of its page; each group looks for
 // them among `tpg` tokens. A run of up to AP_REGS float4 per thread stays in registers between the maximum
 // and the rounding, a larger one is read again (from L1 or L2). Bound by memory; with a warp for every run
 // and two reads, prompts of 7 k tokens into pages of 128 took 120 us.
@@ -321,21 +329,21 @@ __global__ void __launch_bounds__(AP_THREADS, 3) append_i8_kernel(const AppendPa
         for (int i0 = gl; i0 < pieces; i0 += TPR * AP_REGS) {
             load(i0);
 #pragma unroll
-            for (int u = 0; u < AP_REGS; ++u) amax = fmaxf(amax, amax4(v[u]));
+            for (int u = 0; u < AP_REGS; ++u) amax = max_nan(amax, amax4(v[u]));
         }
 #pragma unroll
-        for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        for (int o = 16; o; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         if constexpr (WARPS > 1) {
             if (lane == 0) s_max[parity][threadIdx.x >> 5] = amax;
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < WARPS; ++i) amax = fmaxf(amax, s_max[parity][i]);
+            for (int i = 0; i < WARPS; ++i) amax = max_nan(amax, s_max[parity][i]);
             parity ^= 1;
         }
         float scale = amax / 127.0f;
         if (rat > 0) {
             const float old = p.scale[which][rb];
-            if (old >= scale) {
+            if (scale == scale && !(old < scale)) {  // (old may be NaN)
                 scale = old;
             } else {
                 const float ratio = __fdiv_rn(old, scale);
