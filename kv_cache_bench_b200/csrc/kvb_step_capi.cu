@@ -66,6 +66,7 @@ int geometry(Attend& a) {
     if (int rc = kvb_device_sms(&sms)) return rc;
     ChunkParams& p = a.p;
     const kvb_shape& s = a.s;
+    p.max_new = std::min(p.max_new, p.T);  // no sequence has more rows than the step, whatever the bound
     p.B = s.batch;
     p.H = s.num_heads;
     p.Hkv = s.num_kv_heads;
