@@ -133,8 +133,9 @@ struct CCfg {
     static constexpr int NBARS = 2 * STAGES + 4 * RAWS + 11 + CU_CLEAN + 2 * CU_RING + SR;
     static constexpr size_t UNIT_OFF = kvb_align_up(BAR_OFF + 8 * NBARS, 64);
     static constexpr size_t SCALE_OFF = UNIT_OFF + 64 * CU_RING;           // [SR tiles][K, V][16 pages]
-    static constexpr size_t VMAX_OFF = SCALE_OFF + (RAWS ? SR * 2 * 16 * 4 : 0);  // [SR tiles]
-    static constexpr size_t MISC_OFF = kvb_align_up(VMAX_OFF + (RAWS ? SR * 4 : 0), 16);
+    // [SR tiles][16 pages]: the largest biased exponent of a finite V scale up to each page
+    static constexpr size_t VMAX_OFF = SCALE_OFF + (RAWS ? SR * 2 * 16 * 4 : 0);
+    static constexpr size_t MISC_OFF = kvb_align_up(VMAX_OFF + (RAWS ? SR * 16 : 0), 16);
     static constexpr size_t SMEM = MISC_OFF + 16 + 4 * CU_CLEAN + 1024;
     static_assert(NK >= 1 && NV >= 1 && SMEM <= 227 * 1024, "shared memory budget");
     static_assert(KV_OFF % 1024 == 0 && RAW_OFF % 1024 == 0, "swizzled tiles need 1024-byte alignment");
@@ -270,7 +271,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
     uint64_t* sc_free = r_empty + CU_RING;  // [SR] int8: both softmax groups are through with the slot's scales
     auto ring = [&](int e) -> RingUnit& { return *reinterpret_cast<RingUnit*>(smem + C::UNIT_OFF + 64 * (e % CU_RING)); };
     float* s_scale = reinterpret_cast<float*>(smem + C::SCALE_OFF);
-    float* s_vmax = reinterpret_cast<float*>(smem + C::VMAX_OFF);
+    uint8_t* s_vmax = smem + C::VMAX_OFF;
     volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::MISC_OFF);
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::MISC_OFF + 8);
     unsigned* s_clean = reinterpret_cast<unsigned*>(smem + C::MISC_OFF + 16);  // [CU_CLEAN] cleaning warps done
@@ -483,7 +484,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             // one (every score so far was -inf). Rows of no token hold anything: they move no reference.
             float most = live ? -1.f : INFINITY;
             float l = 0.f;
-            float vexp = 0.f;       // int8: 2^-e, probabilities times the value scales times this; 0: not set
+            float vexp = 0.f;       // int8: 2^-e, probabilities times the value scales times this; 0: not set yet
             float older = 1.f;      // what the folded sum has to be scaled by
             int folds = 0;
             // every value product of this tile so far is done
@@ -575,12 +576,17 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                         older = 1.f;
                     }
                     if constexpr (SRC == SRC_I8) {
-                        const float vm = s_vmax[(tiles + j) % C::SR];  // the tile's largest finite value scale
-                        if (vexp == 0.f || vm * vexp > 2.f) {          // (the same in every row)
-                            const int x = min(max(int(__float_as_uint(vm) >> 23) - 127, -100), 125);
-                            const float ve = __uint_as_float(uint32_t(126 - x) << 23);  // vm * ve in [0.5, 1)
-                            if (vexp != 0.f) rescale(ve / vexp);
-                            vexp = ve;
+                        // the largest value scale among the pages that this row sees (a larger one behind them would
+                        // push the row's probabilities out of fp16's range), down to a power of two
+                        const int last = masked ? (min(limit - k0, CU_ROWS) - 1) >> lp : 15;
+                        const int vm = last >= 0 ? s_vmax[(tiles + j) % C::SR * 16 + last] : 0;
+                        const bool move = vexp == 0.f || __uint_as_float(uint32_t(vm) << 23) * vexp > 1.f;
+                        // (the rows differ in masked tiles only, which are a unit's last)
+                        if (masked ? __any_sync(0xffffffffu, move) != 0 : move) {
+                            // times the scale in [0.5, 1)
+                            const float ve = __uint_as_float(uint32_t(253 - min(max(vm, 27), 252)) << 23);
+                            if (j > 0) rescale(move ? ve / vexp : 1.f);
+                            if (move) vexp = ve;
                         }
                     }
                 };
@@ -1021,12 +1027,18 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                         const float vs = ok ? __ldg(p.v_scale + (long long)id * p.Hkv + u.kvh) : 0.f;
                         if (item >= RAWS) wait(&rk_empty[st], item / RAWS - 1);
                         if (item >= C::SR) wait(&sc_free[item % C::SR], item / C::SR - 1);
-                        const float vm = warp_max(vs <= 3.402823466e38f ? vs : 0.f);
+                        int vm = __float_as_uint(vs) >> 23 & 255;  // its exponent, of finite ones
+                        vm = vm < 255 ? vm : 0;
+#pragma unroll
+                        for (int o = 1; o < 16; o <<= 1) {
+                            const int x = __shfl_up_sync(0xffffffffu, vm, o);
+                            if (lane >= o) vm = max(vm, x);
+                        }
                         if (lane < 16) {
                             s_scale[item % C::SR * 32 + lane] = ks;
                             s_scale[item % C::SR * 32 + 16 + lane] = vs;
+                            s_vmax[item % C::SR * 16 + lane] = uint8_t(vm);
                         }
-                        if (lane == 0) s_vmax[item % C::SR] = vm;
                         __syncwarp();
                         load_tile(u, tile, id, false, st, &rk_full[st], ring(e));
                     } else {
