@@ -5,7 +5,7 @@ import torch
 
 import kv_cache_bench_b200 as kvb
 from kv_cache_bench_b200 import torch_ops as ops
-from tests.step_cases import F16, F32, attention64, ints, make_cache, make_q, rows_of, starts, tolerance
+from tests.step_cases import F16, F32, I8, attention64, ints, make_cache, make_q, rows_of, starts, tolerance
 
 pytestmark = pytest.mark.gpu
 AUTO, SIMT = kvb.Kernel.auto, kvb.Kernel.simt
@@ -84,3 +84,25 @@ def test_infinite_keys(kernel, qt, kv, D, G, n, ctx, at):
     assert want[:, 2 * G - 1].isfinite().any()
     same(o, want, qt)
     assert torch.equal(o.nan_to_num(7), run().nan_to_num(7))
+
+
+@pytest.mark.parametrize("kernel", [AUTO, SIMT])
+@pytest.mark.parametrize("qt,kv", [(F16, F16), (F32, F16), (F16, I8), (F32, I8), (F32, F32)])
+@pytest.mark.parametrize("new,ctx", [([150], [100]), ([3, 40], [3000, 0])])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_nonfinite_queries_stay_in_their_rows(kernel, qt, kv, new, ctx, bad):
+    c = make_cache(new, ctx, 2, 128, 16, kv, seed=5)
+    q = make_q(sum(new), 8, 128, qt, 6)
+    a = ops.PagedPrefill()
+
+    def run():
+        return a.chunk(q, c["k"], c["v"], c["table"], ints(c["total"]), starts(new), max_new=max(new),
+                       max_len=max(c["total"]), k_scale=c["ks"], v_scale=c["vs"], kernel=kernel)
+
+    want = run().double()
+    rows = torch.zeros(sum(new), 8, dtype=torch.bool, device="cuda")
+    rows[::3, 1] = rows[1, 5] = rows[sum(new) - 1, 7] = True
+    q[rows] = torch.where(torch.arange(128, device="cuda") == 77, bad, q[rows])
+    o = run()
+    assert o[rows].isnan().all()  # (an infinite component scores +inf against some key, and NaN follows)
+    assert (o[~rows].double() - want[~rows]).abs().max().item() <= 2 * tolerance(qt)

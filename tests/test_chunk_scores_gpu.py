@@ -182,3 +182,42 @@ def test_a_prompt_whose_first_keys_score_infinitely_low(dt, D):
         want = attention64(q, k.double(), v.double(), 0)
         assert o[:140].isnan().all() and want[:140].isnan().all()
         assert (o[140:].double() - want[140:]).abs().max().item() <= tolerance(dt)
+
+
+TYPES = [(F16, F16), (F32, F16), (F16, I8), (F32, I8), (F32, F32), (F16, F32)]
+
+
+@pytest.mark.parametrize("kernel", [AUTO, SIMT])
+@pytest.mark.parametrize("qt,kv", TYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("step", [10, 50, 150, 400])
+@pytest.mark.parametrize("every", [1, 40, 128, 200])
+def test_rising_scores(kernel, qt, kv, D, step, every):
+    """... from key to key, tile to tile and in between, in whole and cut units."""
+    check([140, 2], [600, 5000], lambda j, n: min(step * (j // every), 450), 8, 2, D, 64, qt, kv, kernel=kernel)
+
+
+@pytest.mark.parametrize("kernel", [AUTO, SIMT])
+@pytest.mark.parametrize("qt,kv", TYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("step", [-10, -150, -400])
+def test_falling_scores(kernel, qt, kv, D, step):
+    check([140, 2], [600, 5000], lambda j, n: max(step * (j // 100), -450), 8, 2, D, 64, qt, kv, kernel=kernel)
+
+
+@pytest.mark.parametrize("kernel", [AUTO, SIMT])
+@pytest.mark.parametrize("qt,kv", TYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("up", [15, 60, 400])
+def test_single_high_scores(kernel, qt, kv, D, up):
+    """One key of every 301, at changing places of the tiles: the later ones a little higher."""
+    check([140, 2], [600, 5000], lambda j, n: up + j / 200 if j % 301 == 300 else 0.0, 8, 2, D, 64, qt, kv, kernel=kernel)
+
+
+@pytest.mark.parametrize("qt,kv", [(F16, F16), (F32, F16), (F16, I8), (F32, I8)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("every,step", [(1000, 10), (2500, 60), (128, 3)])
+def test_rising_scores_over_folded_sums(qt, kv, D, every, step):
+    """CTAs that take more than 64 key tiles of a unit (38 k keys by 64 heads over at most 148 CTAs are 130 tiles each):
+    the sums that left tensor memory follow the reference."""
+    check([250, 256], [19000, 18800], lambda j, n: min(step * (j // every), 450), 64, 64, D, 128, qt, kv)
