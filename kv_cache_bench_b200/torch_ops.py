@@ -106,6 +106,11 @@ def _type(name: str, t) -> int:
     return k
 
 
+def _bound(n) -> int:
+    """A bound on lengths as the C int it is passed in: any larger one says as much as the largest."""
+    return max(-1, min(int(n), 0x7fffffff))
+
+
 def _tensor(name: str, t, dtype, index: int, shape) -> int:
     """The address of a contiguous tensor of this type, device and shape."""
     if t.dtype is not dtype or t.get_device() != index or t.shape != shape or not t.is_contiguous():
@@ -160,8 +165,10 @@ def plan_step(seq_lens, new_lens, block_table, ring, ring_pos, *, page_size: int
     if index < 0:
         raise ValueError("plan_step takes CUDA tensors")
     page_size, num_blocks, num_tokens = int(page_size), int(num_blocks), int(num_tokens)
-    if num_tokens < 0 or seq_lens.dim() != 1 or ring.dim() != 1:
-        raise ValueError("num_tokens < 0, or seq_lens or ring not one-dimensional")
+    if not 0 <= num_tokens < 1 << 31 or seq_lens.dim() != 1 or ring.dim() != 1:
+        raise ValueError("num_tokens outside [0, 2^31), or seq_lens or ring not one-dimensional")
+    if not 0 < page_size < 1 << 31:
+        raise ValueError("page_size must be in [1, 2^31)")
     batch = seq_lens.shape[0]
     lens = _tensor("seq_lens", seq_lens, _INT32, index, (batch,))
     pos = _tensor("ring_pos", ring_pos, _INT64, index, (2,))
@@ -263,7 +270,7 @@ class PagedPrefill:
         ks = None if k_scale is None else _tensor("k_scale", k_scale, _F32, index, pool[:2])
         vs = None if v_scale is None else _tensor("v_scale", v_scale, _F32, index, pool[:2])
         a = _CChunkArgs(_CShape(batch, H, pool[1], D), _type("q", q), _type("pool", k_pool), pool[2], max_blocks, T,
-                        int(max_new), int(max_len), q.data_ptr(), q_stride,
+                        _bound(max_new), _bound(max_len), q.data_ptr(), q_stride,
                         _tensor("k_pool", k_pool, k_pool.dtype, index, pool),
                         _tensor("v_pool", v_pool, k_pool.dtype, index, pool), ks, vs, pool[0], table,
                         _tensor("total_lens", total_lens, _INT32, index, (batch,)),
@@ -284,7 +291,7 @@ class PagedPrefill:
         T, H, D = q.shape
         if out is None:
             out = q.new_empty(q.shape)
-        a = _CPromptArgs(_CShape(cu_lens.shape[0] - 1, H, k.shape[1], D), _type("q", q), T, int(max_len), q.data_ptr(),
+        a = _CPromptArgs(_CShape(cu_lens.shape[0] - 1, H, k.shape[1], D), _type("q", q), T, _bound(max_len), q.data_ptr(),
                          k.data_ptr(), v.data_ptr(), q_stride, k_stride, v_stride,
                          _tensor("cu_lens", cu_lens, _INT32, index, (cu_lens.shape[0],)),
                          _tensor("out", out, q.dtype, index, q.shape), self.error_word.data_ptr(), kernel)

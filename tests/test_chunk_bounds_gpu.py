@@ -56,3 +56,28 @@ def test_workspace():
                                       block_table=0x4000, total_lens=0x5000, cu_new=0x6000, out=0x8000, error_word=0x7000)
                 sizes.append(kvb.paged_chunk_workspace_bytes(args))
             assert sizes[0] == sizes[1] == sizes[2] < 1 << 32
+
+
+@pytest.mark.parametrize("bound", [2 ** 31, 2 ** 31 + 5, 2 ** 32 + 3, 2 ** 40])
+def test_bounds_beyond_a_c_int(bound):
+    new, ctx = [1, 30], [90, 3]
+    c = make_cache(new, ctx, 2, 64, 16, F16, 2)
+    q = make_q(31, 4, 64, F16, 3)
+    a = ops.PagedPrefill()
+    args = (q, c["k"], c["v"], c["table"], ints(c["total"]), starts(new))
+    x = a.chunk(*args, max_new=bound, max_len=bound)
+    y = a.chunk(*args, max_new=2 ** 31 - 1, max_len=2 ** 31 - 1)
+    assert torch.equal(x, y) and a.error_flag() == 0
+    x = a.prompt(q, q[:, :2], q[:, 2:], starts(new), max_len=bound)
+    assert x.isfinite().all() and a.error_flag() == 0
+    for bad in (0, -1, -2 ** 32 + 50):
+        with pytest.raises(ValueError):
+            a.chunk(*args, max_new=bad, max_len=100)
+        with pytest.raises(ValueError):
+            a.prompt(q, q[:, :2], q[:, 2:], starts(new), max_len=bad)
+    with pytest.raises(ValueError):
+        a.chunk(*args, max_new=30, max_len=-2 ** 32 + 100)
+    for page in (0, -16, 2 ** 32 + 16, 2 ** 31):
+        with pytest.raises(ValueError):
+            ops.plan_step(ints([0]), ints([1]), ints([[0]]), ints([0]), ints([0, 1], torch.int64), page_size=page,
+                          num_blocks=1, num_tokens=1)
