@@ -122,7 +122,7 @@ def _rows(name: str, t, index: int) -> int:
     """The token stride of [tokens][heads][dim] rows; a token's own values lie together."""
     if t.dim() == 3 and t.get_device() == index:
         a, b, c = t.stride()
-        if c == 1 and b == t.shape[2]:
+        if c == 1 and (b == t.shape[2] or t.shape[1] == 1):
             return a
     raise ValueError(f"{name} must be [tokens][heads][dim] on cuda:{index}, with each token's heads contiguous")
 
