@@ -480,9 +480,10 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                 }
             }
             float ref = -INFINITY;  // probabilities are 2^(f s - ref)
-            // What a key tile's probabilities may sum to before the reference moves: anything at all until there is
-            // one (every score so far was -inf). Rows of no token hold anything: they move no reference.
-            float most = live ? -1.f : INFINITY;
+            const float most = live ? CU_MOST : INFINITY;  // rows of no token hold anything: they move no reference
+            // Until a row has a reference (every score so far was -inf) the first finite score has to move it: with
+            // the largest number in its place such a score's probability is inf, and that of -inf 0.
+            auto minus_ref = [&]() { return ref == -INFINITY ? 3.402823466e38f : -ref; };
             float l = 0.f;
             float vexp = 0.f;       // int8: 2^-e, probabilities times the value scales times this; 0: not set yet
             float older = 1.f;      // what the folded sum has to be scaled by
@@ -638,8 +639,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                                     if (up > ref) {
                                         scale = ref == -INFINITY ? 0.f : ex2(ref - up);
                                         ref = up;
-                                        if (live) most = CU_MOST;
-                                        l *= scale;
+                                            l *= scale;
                                         sum *= scale;
                                     }
                                     if (j > 0) rescale(scale);
@@ -655,7 +655,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                                         tc_st16(tp + c, w);
                                     }
                                 }
-                                const float base = ref == -INFINITY ? 0.f : -ref;
+                                const float base = minus_ref();
                                 const uint64_t f2 = pack2(f, f), b2 = pack2(base, base);
                                 uint64_t l0 = 0, l1 = 0;
                                 float vs = 0.f;
@@ -730,7 +730,7 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                     settled();  // the product that reads the probabilities before these
                     // The probabilities to tensor memory; their sum.
                     auto probabilities = [&]() {
-                        const float base = ref == -INFINITY ? 0.f : -ref;
+                        const float base = minus_ref();
                         const uint64_t b2 = pack2(base, base);
                         uint64_t f2 = pack2(f, f), v2 = 0;
                         uint64_t l0 = 0, l1 = 0;
@@ -792,7 +792,6 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
                             if (top > ref) {
                                 scale = ref == -INFINITY ? 0.f : ex2(ref - top);
                                 ref = top;
-                                if (live) most = CU_MOST;
                                 l *= scale;
                             }
                             if (j > 0) rescale(scale);
