@@ -19,7 +19,9 @@ constexpr int SM_KEYS = 32;             // keys of a tile
 // cg), 16 x 8, holds scores of rows rg + 16 i and keys cg + 8 j (4 x 4) and the outputs of the same
 // rows, dims 4 (cg + 8 c) .. + 3. Rows of the shared tiles are padded by four floats, so that the rows
 // a warp reads together lie in different banks. 16 shared-memory loads of 16 bytes feed 256 FMAs of a
-// thread, with a wavefront each: bound by the FMA rate.
+// thread, with a wavefront each, half of the FMAs' time. Bound by latency: a tile's table read, row pointers,
+// loads and three barriers follow one another, with eight warps on an SM and nothing of the next tile on its way
+// (2 x 61 tokens on 451, 32 heads of 128: 58 us, 13 at the FMA rate; a prompt of 1024: 359, 125).
 template <int D>
 struct SimtCfg {
     static constexpr int LD = D + 4;

@@ -8,7 +8,8 @@
 //     P = exp2(f S - m), l += row sums
 //     O[128 rows x D] += P V              (P in tensor memory, V in shared memory, MN-major)
 // with the running reference m of a row raised only when a tile's probabilities sum to more than 2^14 (then O
-// and l are scaled in place), so O stays in tensor memory and the common tile needs no maximum. One
+// and l are scaled in place), so O stays in tensor memory and the common tile needs no maximum; a row without a
+// reference yet is raised by its first finite score. One
 // persistent CTA per SM, 16 warps:
 //   0-3, 4-7   softmax of query tiles 0 and 1, one thread per row (tensor-memory lane).
 //   8          unit scheduler, and TMA producer of the key tiles and the query tiles.
@@ -26,13 +27,17 @@
 // bits; q prescaled per row by a power of two) and both products run on both halves.
 //
 // What bounds it: at head dim 128 the four products of a pair of query tiles take 2048 cycles a key tile and
-// the exponentials as many, and under load the 1 kW power cap lowers the clock, so that the cap on sustained
-// library products (1375 of 1653 TFLOP/s) is the mark. A prompt of 8192 tokens (32 heads over 8, 0.55 TFLOP
-// that count): 445 us, 1240 TFLOP/s; 2048 tokens on a 32 k context: 920 us, 1160 TFLOP/s; 512 fp32 queries on
-// 32 k of int8 pages: 601 us, 910 TFLOP/s of the products with split operands (fp16 queries: 460 us; fp16
-// pages: 250 us. Converting the tiles and their scales are more code than the instruction cache holds beside
-// the rest). Few tokens on long contexts are bound by memory and by the loads in flight (8 ragged chunks, 311 MB: 75 us, 4.1 TB/s) and, at the smallest, by
-// the start, first loads and the join (4 x 3-8 tokens on 4 k, 57 MB: 28 us).
+// the exponentials as many, and a pair takes about 3700: neither pipe is full (55 %), since a tile's
+// probabilities are handed over once and its value product starts behind the last of them. A prompt of 8192
+// tokens (32 heads over 8, 0.55 TFLOP that count): 447-459 us in a burst and 520 in a loop of seconds, whose
+// clock the 1 kW power cap lowers (1230 and 1060 TFLOP/s; library products 1653 and 1375); 2048 tokens on a
+// 32 k context: 904 and 1075 us (1180 and 990 TFLOP/s); 512 fp32 queries on 32 k of int8 pages: 630 and 619
+// us, 870 TFLOP/s of the products with split operands (fp16 queries: 475 us; fp16 pages: 243 us. Converting
+// the tiles and their scales are more code than the instruction cache holds beside the rest). Few tokens on
+// long contexts are bound by a tile's chain of scores, exponentials and value product, with one of the two
+// softmax groups idle in units of one query tile (8 ragged chunks, 311 MB: 76 us, 4.1 TB/s, on pages of 16 and
+// of 128 tokens alike) and, at the smallest, by the start, first loads and the join (4 x 3-8 tokens on 4 k, 57
+// MB: 28 us).
 #include <cuda.h>
 #include <cuda_fp16.h>
 
@@ -60,7 +65,7 @@ enum { SRC_F16 = 0, SRC_I8 = 1, SRC_PACKED = 2 };
 // one direction. So O is added into an fp32 sum in the workspace (rounded to nearest) and started anew
 // every so many key tiles: often for fp32 results, rarely for fp16 ones. (512 fp32 queries on 32 k int8:
 // relative error 3.5e-5 and 3.5e-6 for the plain fp32 form; folded every 8, 12, 16 tiles 3.6e-6, 4.5e-6,
-// 5.6e-6 and 647, 609, 605 us.)
+// 5.6e-6 and 647, 609, 605 us: 12 trades 1e-6 of error for 6 % of the time.)
 constexpr int CU_FOLD_F32 = KVB_CHUNK_FOLD_F32, CU_FOLD_F16 = KVB_CHUNK_FOLD_F16;
 // A row's highest score at its reference's last move has probability 2^CU_SHIFT, so that small ones stay normal
 // in fp16.
