@@ -898,7 +898,10 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
             const bool wanted = SRC != SRC_PACKED && lane * bt < CU_ROWS && k < u.keys;
             const bool ok = wanted && id >= 0 && id < p.num_blocks;
             if (wanted && !ok) atomicMin(&R.bad, k);
-            const uint32_t boxes = SRC == SRC_PACKED ? 1 : __popc(__ballot_sync(0xffffffffu, ok));
+            // A refused page of fp16 rows is a box before the pool's first row, which loads as zeros (int8: its scales
+            // are 0). What shared memory held before could move the reference of rows beside those that see it.
+            const bool loads = SRC == SRC_I8 ? ok : wanted;
+            const uint32_t boxes = SRC == SRC_PACKED ? 1 : __popc(__ballot_sync(0xffffffffu, loads));
             const uint32_t bytes = SRC == SRC_I8 ? uint32_t(bt) * D : uint32_t(bt) * 128 * NSUB;  // of a box
             const bool off = *s_abort != 0;
             if (lane == 0) {
@@ -920,8 +923,8 @@ __global__ void __launch_bounds__((CCfg<SRC, QF32, D>::THREADS), 1)
 #pragma unroll
                         for (int s = 0; s < NSUB; ++s)
                             tma_load_3d(dst + s * CU_SUB, map, done, 64 * s, u.kvh, u.kv0 + tile * CU_ROWS);
-                } else if (ok) {
-                    const int y = (id * p.Hkv + u.kvh) * p.page + k % p.page;
+                } else if (loads) {
+                    const int y = ok ? (id * p.Hkv + u.kvh) * p.page + k % p.page : -bt;
 #pragma unroll
                     for (int s = 0; s < NSUB; ++s)
                         tma_load_2d(dst + s * CU_SUB + lane * bt * 128, map, done, 64 * s, y);

@@ -38,3 +38,30 @@ def test_a_bad_page_reaches_the_tokens_that_see_it(kernel, qt, kv, H, Hkv, D, pa
     assert (o[fine].double() - want[fine]).abs().max().item() <= tolerance(qt) if fine.any() else True
     for _ in range(5):
         assert torch.equal(run()[fine], o[fine])
+
+
+@pytest.mark.parametrize("qt,kv", [(F16, F16), (F32, F16), (F16, I8), (F32, I8)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new,ctx,at", [([200], [300], 400), ([60], [3000], 3030), ([256], [0], 130)])
+def test_what_ran_before_does_not_show_in_the_rows_beside_nan_ones(qt, kv, D, new, ctx, at):
+    """Shared memory that the refused page was not loaded into holds keys of the call before, of any size."""
+    c = make_cache(new, ctx, 2, D, 16, kv, seed=3)
+    q = make_q(sum(new), 4, D, qt, 4) * 3
+    c["table"][0, at // 16] = -1
+    x = make_cache([500] * 4, [200] * 4, 2, D, 16, kv, seed=6)
+    other = make_q(2000, 4, D, qt, 5)
+    if kv is not I8:
+        keys = [x["k"].nan_to_num(0.0) * s for s in (0.001, 3.0, 3000.0)]
+    else:
+        keys = [x["k"] // 2, x["k"], x["k"] * 0]
+    a = ops.PagedPrefill()
+    outs = []
+    for i in range(12):
+        a.chunk(other, keys[i % 3], x["v"], x["table"], ints(x["total"]), starts([500] * 4), max_new=500, max_len=700,
+                k_scale=x["ks"], v_scale=x["vs"])
+        outs.append(a.chunk(q, c["k"], c["v"], c["table"], ints(c["total"]), starts(new), max_new=max(new),
+                            max_len=c["total"][0], k_scale=c["ks"], v_scale=c["vs"]))
+    first = at // 16 * 16 - ctx[0]
+    assert outs[0][:first].isfinite().all() and outs[0][first:].isnan().all()
+    for o in outs[1:]:
+        assert torch.equal(o[:first], outs[0][:first])
